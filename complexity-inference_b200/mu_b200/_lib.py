@@ -58,6 +58,18 @@ SIGNATURES = {
                                              c_int, _P]),
     "muk_paged_prefill_attn": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, c_int, _P, _P, c_int,
                                        c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P]),
+    "muk_rope_kv_append_fp8": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, _P, c_int, c_int,
+                                       c_int, c_int, c_int, _P, _P, c_float, _P, _P, _P, _P, c_int,
+                                       c_int, _P]),
+    "muk_decode_attn_fp8_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "muk_paged_decode_attn_fp8": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int, _P,
+                                          c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                                          _P, c_size_t, _P]),
+    "muk_paged_prefill_attn_fp8": (c_int, [_P, c_int64, _P, c_int64, _P, _P, _P, _P, _P, c_int, _P,
+                                           _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                           c_int, c_int, c_float, _P]),
+    "muk_copy_pages": (c_int, [_P, c_int64, c_int, c_int64, _P, c_int64, c_int, c_int, _P, _P,
+                               c_int, _P]),
     "muk_gemm_bf16": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int, c_int, c_int,
                               c_int, _P, _P]),
     "muk_gemm_plan_split": (c_int, [c_int, c_int, c_int, c_int, c_int]),
@@ -187,7 +199,8 @@ _lib: ctypes.CDLL | None = None
 # Kernel launches issued through call() (entry points that launch two kernels
 # count both); the benchmark reports it as its launch count.
 launch_count = 0
-_TWO_KERNELS = {"muk_paged_decode_attn", "muk_paged_decode_attn_static", "muk_allreduce_f32",
+_TWO_KERNELS = {"muk_paged_decode_attn", "muk_paged_decode_attn_static",
+                "muk_paged_decode_attn_fp8", "muk_allreduce_f32",
                 "muk_gemm_allreduce_f32", "muk_ep_gather_bf16", "muk_tp_residual_norm",
                 "muk_gemm_tp_residual_norm", "muk_tp_allgather_cols", "muk_tp_greedy"}
 

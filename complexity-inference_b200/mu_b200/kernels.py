@@ -8,9 +8,11 @@ sm_100a kernels.  Errors surface as :class:`mu_b200._lib.MukError`.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 from dataclasses import dataclass
+from typing import Sequence
 
 import torch
 
@@ -22,7 +24,8 @@ __all__ = [
     "embed", "residual_rmsnorm", "rmsnorm_rows", "rope_kv_append", "decode_attn_workspace_size",
     "decode_attn", "prefill_attn", "gemm", "grouped_gemm", "route_permute", "gather_rows",
     "inl_dynamics", "reduce_clamp", "sample", "mark_seen", "fill_decode_inputs", "gemm_plan_info",
-    "gemm_set_stream_k", "gemm_qkv_rope",
+    "gemm_set_stream_k", "gemm_qkv_rope", "rope_kv_append_fp8", "decode_attn_fp8",
+    "decode_attn_fp8_workspace_size", "prefill_attn_fp8", "copy_pages",
 ]
 
 
@@ -173,6 +176,198 @@ def prefill_attn(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_ca
          _p(k_cache), _p(v_cache), _p(block_tables), block_tables.stride(0), _p(seq_lens),
          _p(cu_seqlens_q), B, max_q_len, num_q_heads, num_kv_heads, head_dim, block_size,
          num_blocks, scale, _stream())
+
+
+# ---------------------------------------------------------------------------
+# 8-bit KV cache: e4m3 codes [num_blocks, Hkv, 16, D] and one f32 scale for each
+# (block, head), [num_blocks, Hkv]; a cached value is code * scale.
+# ---------------------------------------------------------------------------
+def _check_here(name: str, *tensors: torch.Tensor | None) -> None:
+    """Every tensor on the current CUDA device: the launch goes to its stream."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: every tensor must be on the current CUDA device (cuda:{dev}), "
+                             f"got one on {t.device}")
+
+
+def _check_cache_fp8(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, num_kv_heads: int, head_dim: int) -> tuple[int, int]:
+    """(num_blocks, block_size) of a layer's 8-bit cache, its types and shapes checked."""
+    shape = k_cache.shape
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"{name}: expected float8_e4m3fn caches, got {k_cache.dtype} / {v_cache.dtype}")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError(f"{name}: expected float32 scales, got {k_scale.dtype} / {v_scale.dtype}")
+    if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != head_dim or v_cache.shape != shape:
+        raise ValueError(f"{name}: caches must be [num_blocks, {num_kv_heads}, block_size, {head_dim}], "
+                         f"got {tuple(shape)} / {tuple(v_cache.shape)}")
+    if k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+        raise ValueError(f"{name}: scales must be {tuple(shape[:2])}, got {tuple(k_scale.shape)} / "
+                         f"{tuple(v_scale.shape)}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise ValueError(f"{name}: caches and scales must be contiguous")
+    return shape[0], shape[2]
+
+
+def _check_index(name: str, t: torch.Tensor, what: str, at_least: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.stride(0) != 1 or t.shape[0] < at_least:
+        raise ValueError(f"{name}: {what} must be contiguous int32 with at least {at_least} entries, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_rows(name: str, t: torch.Tensor, what: str, rows: int, width: int) -> int:
+    """Row stride of a [rows.., width..] bf16 tensor."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: {what} must be bfloat16, got {t.dtype}")
+    if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < rows or t.shape[1] < width:
+        raise ValueError(f"{name}: {what} must be [>= {rows}, >= {width}] with contiguous rows, got "
+                         f"{tuple(t.shape)}")
+    return t.stride(0)
+
+
+def _check_tables(name: str, bt: torch.Tensor, rows: int) -> int:
+    if bt.dtype != torch.int32 or bt.dim() != 2 or bt.stride(1) != 1 or bt.shape[0] < rows:
+        raise ValueError(f"{name}: block_tables must be int32 [>= {rows}, blocks] with contiguous rows, "
+                         f"got {bt.dtype} {tuple(bt.shape)}")
+    return bt.shape[1] if bt.shape[0] <= 1 else bt.stride(0)
+
+
+def rope_kv_append_fp8(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
+                       rope_cos: torch.Tensor, rope_sin: torch.Tensor, num_q_heads: int,
+                       num_kv_heads: int, head_dim: int, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       q_norm_w: torch.Tensor | None = None, k_norm_w: torch.Tensor | None = None,
+                       qk_eps: float = 1e-6, num_tokens: int | None = None,
+                       q_out: torch.Tensor | None = None):
+    """:func:`rope_kv_append` into the 8-bit cache: q rows (QK-norm, RoPE) go to
+    ``q_out`` (None: in place), k and v rows are quantised into their blocks, whose
+    scales grow as needed (a block starts anew with its row 0).  Rows of one block
+    must be neighbours in the batch; slots < 0 are skipped."""
+    name = "rope_kv_append_fp8"
+    num_blocks, block_size = _check_cache_fp8(name, k_cache, v_cache, k_scale, v_scale,
+                                              num_kv_heads, head_dim)
+    T = qkv.shape[0] if num_tokens is None else num_tokens
+    q = qkv if q_out is None else q_out
+    ld = _check_rows(name, qkv, "qkv", T, (num_q_heads + 2 * num_kv_heads) * head_dim)
+    ldq = _check_rows(name, q, "q_out", T, num_q_heads * head_dim)
+    _check_index(name, positions, "positions", T)
+    _check_index(name, slot_mapping, "slot_mapping", T)
+    for t in (rope_cos, rope_sin):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != head_dim // 2 \
+                or not t.is_contiguous() or t.shape[0] != rope_cos.shape[0]:
+            raise ValueError(f"{name}: RoPE tables must be contiguous float32 [positions, "
+                             f"{head_dim // 2}]")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != head_dim
+                              or not w.is_contiguous()):
+            raise ValueError(f"{name}: norm weights must be contiguous float32 [{head_dim}]")
+    _check_here(name, qkv, q, positions, slot_mapping, rope_cos, rope_sin, k_cache, v_cache,
+                k_scale, v_scale, q_norm_w, k_norm_w)
+    call("muk_rope_kv_append_fp8", qkv.data_ptr(), ld, q.data_ptr(), ldq, positions.data_ptr(),
+         slot_mapping.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], T,
+         num_q_heads, num_kv_heads, head_dim, _p(q_norm_w), _p(k_norm_w), qk_eps,
+         k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+         num_blocks, block_size, _stream())
+
+
+def decode_attn_fp8_workspace_size(num_seqs: int, num_q_heads: int, head_dim: int,
+                                   max_seq_len: int, block_size: int = 16) -> int:
+    return int(_lib.load().muk_decode_attn_fp8_workspace_size(num_seqs, num_q_heads, head_dim,
+                                                              max_seq_len, block_size))
+
+
+def decode_attn_fp8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                    block_tables: torch.Tensor, seq_lens: torch.Tensor, num_q_heads: int,
+                    num_kv_heads: int, head_dim: int, max_seq_len: int,
+                    workspace: torch.Tensor | None = None, scale: float | None = None,
+                    num_seqs: int | None = None):
+    """:func:`decode_attn` over the 8-bit cache (zero rows for empty sequences).
+    ``workspace``: at least :func:`decode_attn_fp8_workspace_size` bytes, not shared
+    with a call that may run at the same time."""
+    name = "decode_attn_fp8"
+    num_blocks, block_size = _check_cache_fp8(name, k_cache, v_cache, k_scale, v_scale,
+                                              num_kv_heads, head_dim)
+    B = seq_lens.shape[0] if num_seqs is None else num_seqs
+    ldq = _check_rows(name, q, "q", B, num_q_heads * head_dim)
+    ldo = _check_rows(name, out, "out", B, num_q_heads * head_dim)
+    bts = _check_tables(name, block_tables, B)
+    if block_tables.shape[1] * block_size < max_seq_len:
+        raise ValueError(f"{name}: block_tables hold {block_tables.shape[1]} blocks, max_seq_len "
+                         f"{max_seq_len} needs more")
+    _check_index(name, seq_lens, "seq_lens", B)
+    _check_here(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, workspace)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError(f"{name}: workspace must be contiguous")
+    call("muk_paged_decode_attn_fp8", q.data_ptr(), ldq, out.data_ptr(), ldo, k_cache.data_ptr(),
+         v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), bts,
+         seq_lens.data_ptr(), B, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+         head_dim ** -0.5 if scale is None else scale, max_seq_len, _p(workspace),
+         0 if workspace is None else workspace.nbytes, _stream())
+
+
+def prefill_attn_fp8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
+                     v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                     cu_seqlens_q: torch.Tensor, max_q_len: int, num_q_heads: int,
+                     num_kv_heads: int, head_dim: int, scale: float | None = None,
+                     num_seqs: int | None = None, max_seq_len: int | None = None):
+    """:func:`prefill_attn` over the 8-bit cache; rows behind the last sequence are
+    left as they are.  ``max_seq_len``: largest context (None: what a block-table row
+    holds)."""
+    name = "prefill_attn_fp8"
+    num_blocks, block_size = _check_cache_fp8(name, k_cache, v_cache, k_scale, v_scale,
+                                              num_kv_heads, head_dim)
+    B = seq_lens.shape[0] if num_seqs is None else num_seqs
+    ldq = _check_rows(name, q, "q", 0, num_q_heads * head_dim)
+    ldo = _check_rows(name, out, "out", 0, num_q_heads * head_dim)
+    bts = _check_tables(name, block_tables, B)
+    room = block_tables.shape[1] * block_size
+    if max_seq_len is None:
+        max_seq_len = room
+    elif room < max_seq_len:
+        raise ValueError(f"{name}: block_tables hold {block_tables.shape[1]} blocks, max_seq_len "
+                         f"{max_seq_len} needs more")
+    _check_index(name, seq_lens, "seq_lens", B)
+    _check_index(name, cu_seqlens_q, "cu_seqlens_q", B + 1)
+    _check_here(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
+                cu_seqlens_q)
+    call("muk_paged_prefill_attn_fp8", q.data_ptr(), ldq, out.data_ptr(), ldo, k_cache.data_ptr(),
+         v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), bts,
+         seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), B, min(q.shape[0], out.shape[0]), max_q_len,
+         max_seq_len, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
+         head_dim ** -0.5 if scale is None else scale, _stream())
+
+
+def copy_pages(pool: torch.Tensor, src: Sequence[int], dst: Sequence[int],
+               scales: torch.Tensor | None = None):
+    """Block ``src[i]`` to block ``dst[i]`` in every plane of ``pool``
+    [..., num_blocks, Hkv, block_size, D] (contiguous, any element type) and of
+    ``scales`` [..., num_blocks, Hkv].  ``src`` / ``dst`` are host integers; no block
+    may be a destination twice, nor a source and a destination."""
+    name = "copy_pages"
+    if pool.dim() < 4 or not pool.is_contiguous():
+        raise ValueError(f"{name}: pool must be a contiguous [..., num_blocks, Hkv, block_size, D]")
+    shape = pool.shape
+    num_blocks, page = shape[-4], shape[-3] * shape[-2] * shape[-1] * pool.element_size()
+    planes = math.prod(shape[:-4])
+    sbytes = 0
+    if scales is not None:
+        if scales.shape != shape[:-2] or not scales.is_contiguous():
+            raise ValueError(f"{name}: scales must be a contiguous {tuple(shape[:-2])}, got "
+                             f"{tuple(scales.shape)}")
+        sbytes = shape[-3] * scales.element_size()
+    s, d = array.array("i", src), array.array("i", dst)
+    if len(s) != len(d):
+        raise ValueError(f"{name}: {len(s)} sources for {len(d)} destinations")
+    _check_here(name, pool, scales)
+    if len(s) == 0:
+        return
+    _lib.call_counted("muk_copy_pages", (len(s) + 255) // 256, pool.data_ptr(), num_blocks * page,
+                      planes, page, _p(scales), num_blocks * sbytes, sbytes, num_blocks,
+                      s.buffer_info()[0], d.buffer_info()[0], len(s), _stream())
 
 
 def gemm(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, epilogue: int = MUK_EPI_BF16,

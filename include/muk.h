@@ -189,6 +189,76 @@ int muk_paged_prefill_attn(const void* q, int64_t q_stride, void* out, int64_t o
                            int num_q_heads, int num_kv_heads, int head_dim, int block_size,
                            int num_blocks, float scale, void* stream);
 
+/* ---- 8-bit KV cache ------------------------------------------------------- */
+
+/* The 8-bit cache of a layer: two arrays [num_blocks][num_kv_heads][16][head_dim]
+ * of e4m3 codes (K and V, 16-byte aligned) and one f32 scale for each (block,
+ * KV head), [num_blocks][num_kv_heads] for K and for V.  A cached value is
+ * code * scale.  Scales lie in [2^-60, 2^60] (the readers clamp to that) or are
+ * NaN: the block then reads as NaN.  head_dim 64 or 128, block_size 16.  The
+ * reference has no 8-bit cache; the entry points follow their bf16 siblings. */
+
+/* muk_rope_kv_append for the 8-bit cache: QK-norm (optional; NULL = off) and
+ * rotate-half RoPE of q and k, q rows to q_out (row stride q_out_stride; may be
+ * qkv itself), k and v quantised into the blocks of slot_mapping (slots < 0 are
+ * skipped).  Per (block, head) that gets rows: with a their largest |x|,
+ * e = the smallest exponent with a <= 448 * 2^e, in [-60, 60]; a block whose row
+ * 0 is among them starts anew, any other keeps its rows: e = max(e, its old
+ * exponent), and where that grew its codes are rounded to the new scale.  The
+ * codes are e4m3(x * 2^-e) and the scale 2^e.  A non-finite x makes the scale
+ * NaN until the block starts anew.  Rows of one block must be neighbours in the
+ * batch (a sequence's new tokens in order); of neighbouring rows naming one slot
+ * the last counts.  qkv / q_out strides multiples of 8, buffers 16-byte aligned.
+ * Bad positions and blocks latch device error 5 and are skipped. */
+int muk_rope_kv_append_fp8(const void* qkv, int64_t qkv_stride, void* q_out, int64_t q_out_stride,
+                           const int32_t* positions, const int32_t* slot_mapping,
+                           const float* rope_cos, const float* rope_sin, int max_pos,
+                           int num_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                           const float* q_norm_w, const float* k_norm_w, float qk_eps,
+                           void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                           int num_blocks, int block_size, void* stream);
+
+/* Scratch bytes muk_paged_decode_attn_fp8 needs for any batch of up to num_seqs
+ * sequences whose contexts are at most max_seq_len (0 if none). */
+size_t muk_decode_attn_fp8_workspace_size(int num_seqs, int num_q_heads, int head_dim,
+                                          int max_seq_len, int block_size);
+
+/* muk_paged_decode_attn over the 8-bit cache.  Sequences with seq_lens[b] <= 0
+ * get zero rows; scale > 0.  Contexts beyond the launch's size and bad block ids
+ * latch device error 5 as there. */
+int muk_paged_decode_attn_fp8(const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                              const void* k_cache, const void* v_cache, const float* k_scale,
+                              const float* v_scale, const int32_t* block_tables,
+                              int block_table_stride, const int32_t* seq_lens, int num_seqs,
+                              int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                              int num_blocks, float scale, int max_seq_len, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* muk_paged_prefill_attn over the 8-bit cache; scale > 0, strides multiples of 8,
+ * q and out 16-byte aligned.  num_rows: rows of q and out; max_seq_len: largest
+ * context, which a block-table row holds.  A sequence whose rows do not lie in
+ * [0, num_rows), whose seq_lens is below its q length or above max_seq_len's
+ * blocks, or with more than max_q_len rows latches device error 4 and is skipped. */
+int muk_paged_prefill_attn_fp8(const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                               const void* k_cache, const void* v_cache, const float* k_scale,
+                               const float* v_scale, const int32_t* block_tables,
+                               int block_table_stride, const int32_t* seq_lens,
+                               const int32_t* cu_seqlens_q, int num_seqs, int num_rows,
+                               int max_q_len, int max_seq_len, int num_q_heads, int num_kv_heads,
+                               int head_dim, int block_size, int num_blocks, float scale,
+                               void* stream);
+
+/* Copies page src[i] to page dst[i] for i < n in each of num_planes planes of a
+ * pool (plane p at pool + p * plane_stride bytes, num_blocks pages of page_bytes;
+ * multiples of 16) and, where scales is not NULL, their block scales (scale_bytes
+ * a page, plane stride scale_plane_stride) in the same launch.  src and dst are
+ * HOST arrays, read before the call returns (a captured graph keeps the pairs of
+ * its capture).  No page may be a destination twice, nor a source and a
+ * destination: MUK_ERR_INVALID_ARG, nothing copied.  Pools of any element type. */
+int muk_copy_pages(void* pool, int64_t plane_stride, int num_planes, int64_t page_bytes,
+                   void* scales, int64_t scale_plane_stride, int scale_bytes, int num_blocks,
+                   const int32_t* src, const int32_t* dst, int n, void* stream);
+
 /* ---- K3: dense GEMM on tcgen05 / TMEM ------------------------------------ */
 
 /* C[M,N] = epilogue(A[M,K] · B[N,K]ᵀ); A and B are bf16, K-major (row-major
