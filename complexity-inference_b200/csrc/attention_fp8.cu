@@ -32,6 +32,7 @@
 #include "abi_util.h"
 #include "common.cuh"
 #include "fp8.cuh"
+#include "prefill_fp8.h"
 
 namespace muk {
 
@@ -427,24 +428,6 @@ static int launch_decode_fp8(DecodeFp8Args a, const DecodeFp8Split& p, int num_s
 constexpr int kQpKeys = 64;
 constexpr int kQpBlocks = kQpKeys / kKvBlock;
 
-struct PrefillFp8Args {
-  const __nv_bfloat16* q;
-  int64_t q_stride;
-  __nv_bfloat16* out;
-  int64_t out_stride;
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
-  const float* k_scale;
-  const float* v_scale;
-  const int32_t* block_tables;
-  int bt_stride;
-  const int32_t* seq_lens;
-  const int32_t* cu_q;
-  int num_q_heads, num_kv_heads, num_blocks;
-  int num_rows, max_q_len, max_blocks;
-  float scale_log2;
-};
-
 // Byte offset of 16-byte chunk c (8 f16) of row r in a staged tile.
 template <int D>
 __device__ __forceinline__ uint32_t swz16(int r, int c) {
@@ -810,6 +793,7 @@ extern "C" int muk_paged_prefill_attn_fp8(const void* q, int64_t q_stride, void*
                   (int64_t)block_table_stride * kKvBlock >= max_seq_len,
               "muk_paged_prefill_attn_fp8: block table narrower than max_seq_len");
   MUK_REQUIRE(num_seqs <= 65535, "muk_paged_prefill_attn_fp8: %d sequences in one call", num_seqs);
+  MUK_REQUIRE(max_q_len <= 8 * 65535, "muk_paged_prefill_attn_fp8: %d rows of a sequence", max_q_len);
   if (num_seqs <= 0 || max_q_len <= 0) return MUK_OK;
   PrefillFp8Args a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
@@ -832,6 +816,8 @@ extern "C" int muk_paged_prefill_attn_fp8(const void* q, int64_t q_stride, void*
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t s = as_stream(stream);
+  if (prefill_fp8_tc_supported(head_dim, num_q_heads, num_kv_heads))
+    return launch_prefill_fp8_tc(a, num_seqs, max_q_len, s);
   return head_dim == 128 ? prefill_fp8<128>(a, num_seqs, max_q_len, s)
                          : prefill_fp8<64>(a, num_seqs, max_q_len, s);
 }
