@@ -8,25 +8,26 @@
 // are rounded to f16 (2^-11, bf16 would be 2^-8).
 //
 // Tile shape.  256 rows = two query tiles of 128 (the G = Hq / Hkv heads of one KV
-// head times 128 / G positions each); keys in tiles of 128.  Two query tiles share
-// every converted K / V tile, which halves the conversion per multiply, and take
-// turns: the tensor core multiplies for one while the softmax of the other runs.
+// head times 128 / G positions each); keys in tiles of 64.  Two query tiles share
+// every converted K / V tile, which halves the conversion per multiply.  With 64
+// keys a query tile has two S buffers beside its O in TMEM (2 x 64 + 128 columns),
+// so S(t + 1) is there when the softmax of t ends: with 128 keys and one buffer a
+// row's chain softmax -> P V -> Q K^T -> softmax took 5,250 clocks per 128 keys, of
+// which the tensor core worked 2,050.
 //
-// Warp roles (12 warps, so that each SM sub-partition holds three of 168 registers):
+// Warp roles (14 warps of up to 128 registers):
 //   0-3, 4-7   softmax of query tile 0 / 1, one thread per row: S from TMEM, mask,
 //              weights back into TMEM over S (f16, the A operand of P V), O / l out.
-//              64 columns are held at a time (the upper half is read twice).
-//   8-10       conversion: 16 codes a load from the paged blocks, f16 into 128-byte
-//              swizzled K-major (K) / MN-major (V) panels, two stages each.  The loads of
-//              the next tile are in flight while this one is converted.
-//   11         TMEM owner; one thread issues PV0(t), QK0(t+1), PV1(t), QK1(t+1), ...
-//              S0(t+1) overwrites P0(t): MMAs of one thread execute in order.
-// TMEM: S0 / P0 0-127, S1 / P1 128-255, O0 256-383, O1 384-511.
+//   8-11       conversion of codes to f16, 16 at a time, into 128-byte swizzled K-major
+//              (K) / MN-major (V) panels, three stages each.
+//   12         TMEM owner; issues PV_i(t), QK_i(t + 2) for i = 0, 1 in turn.
+//              S_i(t + 2) overwrites P_i(t): MMAs of one thread execute in order.
+//   13         copies the paged blocks' codes (2 KB each, cp.async.bulk) into a ring.
+// TMEM: S_i of tile t at 128 i + 64 (t & 1), O_i at 256 + 128 i.
 //
 // The running bound only moves when a tile exceeds it by more than 8, so weights
-// stay below 2^8 and O is rescaled in TMEM on those tiles alone; O and l use the
-// same bound.  By the time S(t) is complete P V of t - 1 is too, so its thread may
-// rescale O without a further barrier.
+// stay below 2^8 and O is rescaled in TMEM on those tiles alone (after P V of the
+// tile before has run); O and l use the same bound.
 //
 // Every wait is bounded (common.cuh); on time-out the kernel records the error
 // word, every role leaves its loop, TMEM is freed and the CTA returns.
@@ -41,26 +42,68 @@ namespace muk {
 
 constexpr int kXD = 128;             // head_dim
 constexpr int kXRows = 128;          // rows of a query tile
-constexpr int kXKeys = 128;          // keys of a tile
-constexpr int kXBlocks = kXKeys / kKvBlock;
-constexpr int kXThreads = 384;
-constexpr int kXConvert = 3;         // conversion warps
-constexpr int kXGroups = 32;         // 512-byte groups (4 rows of codes) of a K or V tile
-constexpr int kXPanel = 128 * 128;   // [128 rows][64 f16], one swizzled panel
+constexpr int kXKeys = 64;           // keys of a tile
+constexpr int kXThreads = 448;
+constexpr int kXConvert = 4;         // conversion warps, after the eight of the softmax
+constexpr int kXIssuer = 12;         // the warp that owns TMEM and issues the multiplies
+constexpr int kXLoader = 13;         // the warp that issues the copies of codes
+constexpr int kXStages = 3;          // converted K tiles, and V tiles
+constexpr int kXRing = 3;            // steps (a V and a K tile) of codes on their way
+constexpr int kXItem = kXKeys * 128; // bytes of such a tile
+constexpr int kXQPanel = 128 * 128;  // [128 rows][64 f16], one swizzled panel of a query tile
+constexpr int kXPanel = kXKeys * 128;  // the same of a K or V tile
 
 struct XLayout {
-  static constexpr int kQ = 0;                               // 2 tiles x 2 panels
-  static constexpr int kK = kQ + 4 * kXPanel;                // 2 stages x 2 panels
-  static constexpr int kV = kK + 4 * kXPanel;
   static constexpr int kStage = 2 * kXPanel;
-  static constexpr int kBar = kV + 4 * kXPanel;
+  static constexpr int kQ = 0;                               // 2 tiles x 2 panels
+  static constexpr int kK = kQ + 4 * kXQPanel;
+  static constexpr int kV = kK + kXStages * kStage;
+  static constexpr int kRaw = kV + kXStages * kStage;
+  static constexpr int kBar = kRaw + kXRing * 2 * kXItem;
   static constexpr int kScale = kBar + 256;                  // [8 warps][2][8 blocks] float4
-  static constexpr int kBytes = kScale + 8 * 2 * kXBlocks * 16 + 1024;  // + alignment slack
+  static constexpr int kRawScale = kScale + 8 * 2 * 8 * 16;  // [8 warps][8 blocks] (ks, vs)
+  static constexpr int kBytes = kRawScale + 8 * 64 + 1024;   // + alignment slack
 };
 static_assert(XLayout::kBytes <= 232448, "prefill tile exceeds 227 KB of shared memory");
 
+// Bounded wait of a whole warp (about a second).  The polls are one loop in PTX: as
+// a C++ loop a wait on a barrier that was complete already took ~250 clocks.
 __device__ __forceinline__ bool x_wait(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+  for (int round = 0; round < 64; ++round) {
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        ".reg .u32 n;\n"
+        "mov.u32 n, 0;\n"
+        "W%=:\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "@p bra D%=;\n"
+        "add.u32 n, n, 1;\n"
+        "setp.lt.u32 q, n, 1048576;\n"
+        "@q bra W%=;\n"
+        "D%=:\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done != 0)) return true;
+    if (*reinterpret_cast<volatile int*>(&g_device_error) != 0) break;
+  }
+  set_device_error(code);  // keeps an earlier code
+  return false;
+}
+__device__ __forceinline__ uint32_t x_elect() {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(r));
+  return r;
 }
 // 2^x, one MUFU op (~2 ulp), far below what the f16 weight keeps.
 __device__ __forceinline__ float x_exp2(float x) {
@@ -68,21 +111,69 @@ __device__ __forceinline__ float x_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// D(tmem) (+)= A(tmem, f16) * B(smem descriptor)
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t accumulate) {
+__device__ __forceinline__ float x_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Largest of 16 raw scores.
+__device__ __forceinline__ float x_max16(const uint32_t* x) {
+  auto f = [&](int i) { return __uint_as_float(x[i]); };
+  const float a = x_max3(f(0), f(1), f(2)), b = x_max3(f(3), f(4), f(5));
+  const float c = x_max3(f(6), f(7), f(8)), d = x_max3(f(9), f(10), f(11));
+  const float e = x_max3(f(12), f(13), f(14));
+  return x_max3(x_max3(a, b, c), x_max3(d, e, f(15)), a);
+}
+// The warp runs the issue loop as one, so that addresses stay in uniform registers
+// (from one diverged lane each multiply took ~80 clocks to issue, more than its 64
+// to run); `lead` picks the lane that issues.
+// D(tmem) (+)= A(smem descriptor) * B(smem descriptor)
+__device__ __forceinline__ void x_mma_ss(uint32_t lead, uint32_t d, uint64_t adesc, uint64_t bdesc,
+                                         uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, q;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
       "}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead));
+}
+// D(tmem) (+)= A(tmem, f16) * B(smem descriptor)
+__device__ __forceinline__ void x_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t bdesc,
+                                         uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "setp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead));
+}
+__device__ __forceinline__ void x_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %1, 0;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+// 16 registers per thread into 32 lanes x 16 columns of TMEM.
+__device__ __forceinline__ void x_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 // Instruction descriptor, kind::f16: f16 A/B (format 0), f32 D, A K-major.
-__host__ __device__ constexpr uint32_t x_idesc(bool b_mn) {
-  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(128 >> 3) << 17) |
-         ((uint32_t)(128 >> 4) << 24);
+__host__ __device__ constexpr uint32_t x_idesc(bool b_mn, int n) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kXRows >> 4) << 24);
 }
 
 __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const PrefillFp8Args a) {
@@ -95,13 +186,16 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* basep = smem_raw + (base - raw);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(basep + XLayout::kBar);
-  uint64_t* k_empty = k_full + 2;
-  uint64_t* v_full = k_empty + 2;
-  uint64_t* v_empty = v_full + 2;
-  uint64_t* s_full = v_empty + 2;   // [2] S of query tile i complete (and its last P V)
-  uint64_t* p_full = s_full + 2;    // [2] weights of query tile i written
-  uint64_t* o_done = p_full + 2;    // [2]
-  uint64_t* q_full = o_done + 2;
+  uint64_t* k_empty = k_full + kXStages;
+  uint64_t* v_full = k_empty + kXStages;
+  uint64_t* v_empty = v_full + kXStages;
+  uint64_t* s_full = v_empty + kXStages;  // [query tile][buffer] S complete
+  uint64_t* p_full = s_full + 4;          // [query tile][buffer] weights written
+  uint64_t* o_done = p_full + 4;          // [query tile] P V of a tile complete
+  uint64_t* o_last = o_done + 2;          // [query tile] P V of the last tile complete
+  uint64_t* raw_full = o_last + 2;        // [ring slot] codes of a step
+  uint64_t* raw_empty = raw_full + kXRing;
+  uint64_t* q_full = raw_empty + kXRing;
   uint64_t* drain = q_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
@@ -128,20 +222,29 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   const int32_t* bt = a.block_tables + (int64_t)b * a.bt_stride;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kXStages; ++i) {
       mbar_init(&k_full[i], kXConvert);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], kXConvert);
       mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&o_done[i], 1);
+      mbar_init(&o_last[i], 1);
+    }
+    for (int i = 0; i < kXRing; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], kXConvert);
     }
     mbar_init(q_full, 8);
     mbar_init(drain, 1);
     fence_mbar_init();
   }
-  if (warp == 11) {
+  if (warp == kXIssuer) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -150,136 +253,178 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 11) {
+  if (warp == kXIssuer) {
     // ---- MMA issuer ---------------------------------------------------------
-    if (lane == 0) {
-      const uint32_t sq = base + XLayout::kQ;
-      auto qk = [&](int i, int t) {  // S_i = Q_i K_t^T
-        const uint32_t sk = base + (uint32_t)(XLayout::kK + (t & 1) * XLayout::kStage);
+    const uint32_t lead = x_elect();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t dq = umma_desc_sw128(base + XLayout::kQ);
+    const uint64_t dk = umma_desc_sw128(base + XLayout::kK);
+    const uint64_t dv = umma_desc_sw128_mn(base + XLayout::kV, kXPanel, 1024);
+    // descriptors count addresses in 16-byte units
+    auto qk = [&](int i, int t) {  // S_i(t) = Q_i K_t^T
+      const uint64_t k0 = dk + (uint64_t)((t % kXStages) * (XLayout::kStage >> 4));
+      const uint32_t d = tm + (uint32_t)(i * 2 * kXKeys + (t & 1) * kXKeys);
 #pragma unroll
-        for (int k = 0; k < kXD / 16; ++k) {
-          const uint32_t off = (uint32_t)((k >> 2) * kXPanel + (k & 3) * 32);
-          tc_mma_f16(tmem + (uint32_t)(i * kXKeys),
-                     umma_desc_sw128(sq + (uint32_t)(i * 2 * kXPanel) + off),
-                     umma_desc_sw128(sk + off), x_idesc(false), k > 0 ? 1u : 0u);
-        }
-        tc_commit(&s_full[i]);
-      };
-      auto pv = [&](int i, int t) {  // O_i += P_i V_t
-        const uint32_t sv = base + (uint32_t)(XLayout::kV + (t & 1) * XLayout::kStage);
+      for (int k = 0; k < kXD / 16; ++k)
+        x_mma_ss(lead, d, dq + (uint64_t)((i * 2 * kXQPanel + (k >> 2) * kXQPanel + (k & 3) * 32) >> 4),
+                 k0 + (uint64_t)(((k >> 2) * kXPanel + (k & 3) * 32) >> 4), x_idesc(false, kXKeys),
+                 k > 0 ? 1u : 0u);
+      x_commit(lead, &s_full[i * 2 + (t & 1)]);
+    };
+    auto pv = [&](int i, int t) {  // O_i += P_i(t) V_t
+      const uint64_t v0 = dv + (uint64_t)((t % kXStages) * (XLayout::kStage >> 4));
+      const uint32_t p = tm + (uint32_t)(i * 2 * kXKeys + (t & 1) * kXKeys);
 #pragma unroll
-        for (int k = 0; k < kXKeys / 16; ++k)
-          tc_mma_f16_ts(tmem + (uint32_t)(2 * kXKeys + i * kXD), tmem + (uint32_t)(i * kXKeys + k * 8),
-                        umma_desc_sw128_mn(sv + (uint32_t)(k * 16 * 128), kXPanel, 1024),
-                        x_idesc(true), (t > 0 || k > 0) ? 1u : 0u);
-      };
-      bool ok = mbar_wait(q_full, 0, kDevTimeoutFull) && mbar_wait(&k_full[0], 0, kDevTimeoutFull);
-      if (ok) {
-        tc_fence_after();
-        qk(0, 0);
-        qk(1, 0);
-        tc_commit(&k_empty[0]);
-      }
-      for (int t = 0; ok && t < nt; ++t) {
-        const bool more = t + 1 < nt;
-        const uint32_t ph = (uint32_t)(t >> 1) & 1u, pn = (uint32_t)((t + 1) >> 1) & 1u;
-        if (!mbar_wait(&v_full[t & 1], ph, kDevTimeoutFull)) break;
-        if (!mbar_wait(&p_full[0], t & 1, kDevTimeoutFull)) break;
-        tc_fence_after();
-        pv(0, t);
-        if (more) {
-          if (!mbar_wait(&k_full[(t + 1) & 1], pn, kDevTimeoutFull)) break;
-          tc_fence_after();
-          qk(0, t + 1);
-        } else {
-          tc_commit(&o_done[0]);
-        }
-        if (!mbar_wait(&p_full[1], t & 1, kDevTimeoutFull)) break;
-        tc_fence_after();
-        pv(1, t);
-        tc_commit(&v_empty[t & 1]);
-        if (more) {
-          qk(1, t + 1);
-          tc_commit(&k_empty[(t + 1) & 1]);
-        } else {
-          tc_commit(&o_done[1]);
-        }
-      }
-      // every MMA this thread issued has finished before TMEM is freed, also
-      // when a wait above gave up
-      tc_commit(drain);
-      mbar_wait(drain, 0, kDevTimeoutAccum);
+      for (int k = 0; k < kXKeys / 16; ++k)
+        x_mma_ts(lead, tm + (uint32_t)(4 * kXKeys + i * kXD), p + (uint32_t)(k * 8),
+                 v0 + (uint64_t)((k * 16 * 128) >> 4), x_idesc(true, kXD), (t > 0 || k > 0) ? 1u : 0u);
+      // a barrier of its own for the last one: its reader may be two tiles ahead of the
+      // multiplies there, which the phase of o_done cannot tell
+      x_commit(lead, t + 1 < nt ? &o_done[i] : &o_last[i]);
+    };
+    bool ok = x_wait(q_full, 0, kDevTimeoutFull);
+    for (int t = 0; ok && t < 2 && t < nt; ++t) {
+      ok = x_wait(&k_full[t], 0, kDevTimeoutFull);
+      if (!ok) break;
+      tc_fence_after();
+      qk(0, t);
+      qk(1, t);
+      x_commit(lead, &k_empty[t]);
     }
-    __syncwarp();
-  } else if (warp >= 8) {
-    // ---- conversion -----------------------------------------------------------
-    // group g (of 32): rows 4g .. 4g + 3 of the tile, 512 contiguous bytes of block g / 4;
-    // lane: row lane / 8 of them, 16-code chunk lane % 8.  Warp w takes g = w, w + 3, ...
-    constexpr int kPer = (kXGroups + kXConvert - 1) / kXConvert;
-    const int w = warp - 8, sub = lane >> 3, c = lane & 7;
-    const int64_t head_off = (int64_t)kvh * (kKvBlock * kXD) + lane * 16;
+    for (int t = 0; ok && t < nt; ++t) {
+      const int n = t + 2;
+      const bool more = n < nt;
+      if (!x_wait(&v_full[t % kXStages], (uint32_t)(t / kXStages) & 1u, kDevTimeoutFull)) break;
+      if (more && !x_wait(&k_full[n % kXStages], (uint32_t)(n / kXStages) & 1u, kDevTimeoutFull)) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ok = x_wait(&p_full[i * 2 + (t & 1)], (uint32_t)(t >> 1) & 1u, kDevTimeoutFull);
+        if (!ok) break;
+        tc_fence_after();
+        pv(i, t);
+        if (i == 1) x_commit(lead, &v_empty[t % kXStages]);
+        if (more) qk(i, n);
+        if (i == 1 && more) x_commit(lead, &k_empty[n % kXStages]);
+      }
+    }
+    // every MMA this warp issued has finished before TMEM is freed, also when a
+    // wait above gave up
+    x_commit(lead, drain);
+    x_wait(drain, 0, kDevTimeoutAccum);
+  } else if (warp == kXLoader) {
+    // ---- loads of codes -------------------------------------------------------
+    // Step t brings V(t) and K(t + 2), which the multiplies of one step need (steps -2
+    // and -1: K alone): lanes 0-3 a block of V each, 4-7 one of K, 2 KB a copy.  Blocks
+    // behind the last key are left out (their rows become zero when converted).
+    const bool mine_k = lane >= 4;
+    const uint8_t* src = (mine_k ? a.k_cache : a.v_cache) + (int64_t)kvh * (kKvBlock * kXD);
     const int64_t blk_bytes = (int64_t)a.num_kv_heads * (kKvBlock * kXD);
-    auto load_ids = [&](int t) {                     // lane j < 8: block j of tile t
-      const int blk = t * kXBlocks + (lane & 7);
-      int id = blk < nblk ? __ldg(bt + blk) : 0;
+    const uint32_t dst = base + (uint32_t)(XLayout::kRaw + (mine_k ? kXItem : 0) + (lane & 3) * 2048);
+    auto block_of = [&](int t) {                     // of this lane in step t, -1: none
+      const int blk = (mine_k ? t + 2 : t) * 4 + (lane & 3);
+      return lane < 8 && blk >= 0 && blk < nblk ? blk : -1;
+    };
+    auto id_of = [&](int t) {
+      const int blk = block_of(t);
+      int id = blk >= 0 ? __ldg(bt + blk) : 0;
       if (id < 0 || id >= a.num_blocks) {
         set_device_error(kDevBadIndex);
         id = 0;
       }
       return id;
     };
-    uint4 v[kPer];
-    int ids = load_ids(0);                           // of the tile being loaded
-    int ids_next = nt > 1 ? load_ids(1) : 0;
-    auto fetch = [&](int g, int t, bool is_v) {      // g < 32, uniform
-      const int64_t id = __shfl_sync(0xffffffffu, ids, g >> 2);
-      // rows behind the last key are zero: what the blocks hold there is not ours
-      if (t * kXKeys + 4 * g + sub < n_keys)
-        return __ldg(reinterpret_cast<const uint4*>((is_v ? a.v_cache : a.k_cache) + id * blk_bytes +
-                                                    head_off + (g & 3) * 512));
-      return make_uint4(0u, 0u, 0u, 0u);
-    };
+    int id = id_of(-2), id_next = id_of(-1), slot = 0, issued = 0;
+    uint32_t ph = 1;
+    for (int t = -2; t < nt; ++t) {
+      if (!x_wait(raw_empty + slot, ph, kDevTimeoutEmpty)) break;
+      const bool have = block_of(t) >= 0;
+      const int blocks = __popc(__ballot_sync(0xffffffffu, have));
+      if (lane == 0) mbar_arrive_expect_tx(raw_full + slot, (uint32_t)(blocks * 2048));
+      __syncwarp();
+      if (have)
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 2048, [%2];\n" ::"r"(
+                dst + (uint32_t)(slot * 2 * kXItem)),
+            "l"(src + id * blk_bytes), "r"(smem_u32(raw_full + slot))
+            : "memory");
+      ++issued;
+      id = id_next;
+      id_next = id_of(t + 2);
+      if (++slot == kXRing) slot = 0, ph ^= 1;
+    }
+    // No copy may still be on its way when the CTA ends, also where the others gave up:
+    // the last copies into each slot have arrived.
+    for (int m = max(issued - kXRing, 0); m < issued; ++m)
+      x_wait(raw_full + m % kXRing, (uint32_t)(m / kXRing) & 1u, kDevTimeoutFull);
+  } else if (warp >= 8) {
+    // ---- conversion -----------------------------------------------------------
+    // Warp w takes rows 4w .. 4w + 3 of every block (512 contiguous bytes), a lane one
+    // 16-code chunk of them.  Eight neighbouring lanes cover two rows of one panel,
+    // which the swizzle puts into all 32 banks.
+    const int w = warp - 8, row = 4 * w + (lane >> 4) * 2 + ((lane >> 2) & 1);
+    const int c = (lane & 3) + ((lane >> 3) & 1) * 4;
+    constexpr int kBpt = kXKeys / kKvBlock;          // blocks of a tile
+    const uint32_t ring = base + (uint32_t)(XLayout::kRaw + row * kXD + c * 16);
+    // this lane's two 16-byte places in block 0's rows of a stage
+    const uint32_t st = base + (uint32_t)((c >> 2) * kXPanel + row * 128);
+    const uint32_t s0 = st + (uint32_t)(((2 * (c & 3)) ^ (row & 7)) << 4);
+    const uint32_t s1 = st + (uint32_t)(((2 * (c & 3) + 1) ^ (row & 7)) << 4);
+    auto read = [&](uint4 (&v)[kBpt], uint32_t src) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (w + kXConvert * j < kXGroups) v[j] = fetch(w + kXConvert * j, 0, false);
-    // chunk pair of a row: the two 16-byte stores of the upper panel's lanes go in
-    // the other order, so that eight lanes of a row hit all 32 banks
-    const uint32_t panel = (uint32_t)((c >> 2) * kXPanel);
-    const int first = c >> 2;
-    bool ok = true;
-    for (int it = 0; ok && it < 2 * nt; ++it) {
-      const int t = it >> 1;
-      const bool is_v = it & 1;
-      uint64_t* empty = is_v ? &v_empty[t & 1] : &k_empty[t & 1];
-      ok = x_wait(empty, (((uint32_t)t >> 1) & 1u) ^ 1u, kDevTimeoutEmpty);
-      if (!ok) break;
-      const int tn = (it + 1) >> 1;                  // tile of the next item
-      if (is_v && tn < nt) {
-        ids = ids_next;
-        if (tn + 1 < nt) ids_next = load_ids(tn + 1);
+      for (int j = 0; j < kBpt; ++j) {
+        const float4 f = ld_shared_f4(src + (uint32_t)(j * 2048));
+        v[j] = make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z),
+                          __float_as_uint(f.w));
       }
-      uint8_t* st = basep + (is_v ? XLayout::kV : XLayout::kK) + (t & 1) * XLayout::kStage + panel;
+    };
+    auto convert = [&](uint4 (&v)[kBpt], int t, uint32_t at) {
+      if (t == nt - 1) {  // rows behind the last key are zero: what the blocks hold there is not ours
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int g = w + kXConvert * j;
-        if (g < kXGroups) {
-          uint32_t x[8];
-          e4m3x4_to_f16x4(v[j].x, x[0], x[1]);
-          e4m3x4_to_f16x4(v[j].y, x[2], x[3]);
-          e4m3x4_to_f16x4(v[j].z, x[4], x[5]);
-          e4m3x4_to_f16x4(v[j].w, x[6], x[7]);
-          if (it + 1 < 2 * nt) v[j] = fetch(g, tn, !is_v);
-          const int r = 4 * g + sub;
-          const uint4 lo = make_uint4(x[0], x[1], x[2], x[3]), hi = make_uint4(x[4], x[5], x[6], x[7]);
-          uint8_t* rowp = st + r * 128;
-          const int c0 = 2 * (c & 3) + first, c1 = 2 * (c & 3) + (first ^ 1);
-          *reinterpret_cast<uint4*>(rowp + ((c0 ^ (r & 7)) << 4)) = first ? hi : lo;
-          *reinterpret_cast<uint4*>(rowp + ((c1 ^ (r & 7)) << 4)) = first ? lo : hi;
-        }
+        for (int j = 0; j < kBpt; ++j)
+          if (t * kXKeys + j * kKvBlock + row >= n_keys) v[j] = make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < kBpt; ++j) {
+        uint32_t x[8];
+        e4m3x4_to_f16x4(v[j].x, x[0], x[1]);
+        e4m3x4_to_f16x4(v[j].y, x[2], x[3]);
+        e4m3x4_to_f16x4(v[j].z, x[4], x[5]);
+        e4m3x4_to_f16x4(v[j].w, x[6], x[7]);
+        const uint32_t o = at + (uint32_t)(j * kKvBlock * 128);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(s0 + o), "r"(x[0]), "r"(x[1]),
+                     "r"(x[2]), "r"(x[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(s1 + o), "r"(x[4]), "r"(x[5]),
+                     "r"(x[6]), "r"(x[7]) : "memory");
+      }
+    };
+    int slot = 0, sg_v = 0, sg_k = 0;
+    uint32_t ph_r = 0;                               // parity of the ring's "full" barriers
+    uint32_t ph_v = 1, ph_k = 1;                     // parities of the stages' "empty" barriers
+    for (int t = -2; t < nt; ++t) {
+      const bool has_v = t >= 0, has_k = t + 2 < nt;
+      uint4 vv[kBpt], vk[kBpt];
+      if (!x_wait(raw_full + slot, ph_r, kDevTimeoutFull)) break;
+      const uint32_t src = ring + (uint32_t)(slot * 2 * kXItem);
+      if (has_v) read(vv, src);
+      if (has_k) read(vk, src + kXItem);
+      if (has_v) {
+        if (!x_wait(v_empty + sg_v, ph_v, kDevTimeoutEmpty)) break;
+        convert(vv, t, (uint32_t)(XLayout::kV + sg_v * XLayout::kStage));
+      }
+      if (has_k) {
+        if (!x_wait(k_empty + sg_k, ph_k, kDevTimeoutEmpty)) break;
+        convert(vk, t + 2, (uint32_t)(XLayout::kK + sg_k * XLayout::kStage));
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(is_v ? &v_full[t & 1] : &k_full[t & 1]);
+      if (lane == 0) {
+        if (has_v) mbar_arrive(v_full + sg_v);
+        if (has_k) mbar_arrive(k_full + sg_k);
+        mbar_arrive(raw_empty + slot);
+      }
+      if (has_v && ++sg_v == kXStages) sg_v = 0, ph_v ^= 1;
+      if (has_k && ++sg_k == kXStages) sg_k = 0, ph_k ^= 1;
+      if (++slot == kXRing) slot = 0, ph_r ^= 1;
     }
   } else {
     // ---- softmax / epilogue: one thread per query row --------------------------
@@ -292,8 +437,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     const int limit = past + pos;                    // last key this row may see
     const int tile_limit = past + p0 + (qi * kXRows + (warp & 3) * 32) / G;  // smallest of the warp
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lane_base + (uint32_t)(qi * kXKeys);
-    const uint32_t to = lane_base + (uint32_t)(2 * kXKeys + qi * kXD);
+    const uint32_t to = lane_base + (uint32_t)(4 * kXKeys + qi * kXD);
     float c;                                          // scale_log2 / the row's power of two
     {
       // the query row, brought into f16 by a power of two
@@ -313,7 +457,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       float up, down;
       row_factor(top, up, down);
       c = down * a.scale_log2;
-      uint8_t* qrow = basep + XLayout::kQ + qi * 2 * kXPanel + r * 128;
+      uint8_t* qrow = basep + XLayout::kQ + qi * 2 * kXQPanel + r * 128;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float2 x0 = unpack_bf16x2(q[i].x), x1 = unpack_bf16x2(q[i].y);
@@ -323,75 +467,82 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
         o.y = pack_f16x2(x1.x * up, x1.y * up);
         o.z = pack_f16x2(x2.x * up, x2.y * up);
         o.w = pack_f16x2(x3.x * up, x3.y * up);
-        *reinterpret_cast<uint4*>(qrow + (i >> 3) * kXPanel + (((i & 7) ^ (r & 7)) << 4)) = o;
+        *reinterpret_cast<uint4*>(qrow + (i >> 3) * kXQPanel + (((i & 7) ^ (r & 7)) << 4)) = o;
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    // Block constants (ks, log2 vs, 1 / vs) of a tile: lanes 0-7 fetch them two
-    // tiles ahead (id, then scales) and leave them in the warp's own buffers.
-    float4* sc = reinterpret_cast<float4*>(basep + XLayout::kScale) + warp * 2 * kXBlocks;
-    auto get_id = [&](int t) {
-      const int blk = t * kXBlocks + (lane & 7);
-      const int id = blk < nblk ? __ldg(bt + blk) : -1;
-      return id < a.num_blocks ? id : 0;             // bad ids are latched by the converters
+    // Block constants (ks, log2 vs, 1 / vs) of two tiles at a time, in the warp's own
+    // buffers: lanes 0-7 read a block's id two pairs ahead and copy its scales one
+    // pair ahead (cp.async: a load into a register would be waited for together with
+    // every other load in flight).
+    float4* sc = reinterpret_cast<float4*>(basep + XLayout::kScale) + warp * 16;
+    const uint32_t raw_sc = base + (uint32_t)(XLayout::kRawScale + warp * 64 + (lane & 7) * 8);
+    auto get_id = [&](int u) {
+      const int blk = u * 8 + (lane & 7);
+      const int id = blk < nblk ? __ldg(bt + blk) : 0;
+      return id >= 0 && id < a.num_blocks ? id : 0;  // bad ids are latched by the converters
     };
-    auto get_scales = [&](int id) {
-      const int64_t at = (int64_t)(id < 0 ? 0 : id) * a.num_kv_heads + kvh;
-      return id < 0 ? make_float2(1.f, 1.f) : make_float2(__ldg(a.k_scale + at), __ldg(a.v_scale + at));
+    auto copy_scales = [&](int id) {
+      const int64_t at = (int64_t)id * a.num_kv_heads + kvh;
+      if (lane < 8) {
+        cp_async_4(raw_sc, a.k_scale + at);
+        cp_async_4(raw_sc + 4, a.v_scale + at);
+      }
+      cp_async_commit();
     };
-    auto put = [&](int t, float2 s) {
-      if (lane < kXBlocks) {
-        const float vs = clamp_scale(s.y);
-        sc[(t & 1) * kXBlocks + lane] = make_float4(clamp_scale(s.x), log2f(vs), 1.f / vs, 0.f);
+    auto put = [&](int u) {
+      cp_async_wait<0>();
+      if (lane < 8) {
+        // blocks behind the last key are hidden from every row, whatever stands here
+        const float ks = clamp_scale(ld_shared_f32(raw_sc)), vs = clamp_scale(ld_shared_f32(raw_sc + 4));
+        float lv, iv;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(vs));   // exact for powers of two
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(iv) : "f"(vs));
+        sc[(u & 1) * 8 + lane] = make_float4(ks, lv, iv, 0.f);
       }
     };
-    put(0, get_scales(get_id(0)));
-    float2 s_next = nt > 1 ? get_scales(get_id(1)) : make_float2(1.f, 1.f);
-    int id_next = nt > 2 ? get_id(2) : -1;
+    const int nu = (nt + 1) >> 1;
+    copy_scales(get_id(0));
+    put(0);
+    if (nu > 1) copy_scales(get_id(1));
+    int id_next = nu > 2 ? get_id(2) : 0;
     __syncwarp();
 
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < nt; ++t) {
-      if (t + 1 < nt) {
-        put(t + 1, s_next);
-        s_next = get_scales(id_next);
-        id_next = t + 3 < nt ? get_id(t + 3) : -1;
+      if ((t & 1) == 0 && (t >> 1) + 1 < nu) {
+        const int u = t >> 1;
+        put(u + 1);
+        if (u + 2 < nu) copy_scales(id_next);
+        if (u + 3 < nu) id_next = get_id(u + 3);
       }
-      ok = x_wait(&s_full[qi], t & 1, kDevTimeoutAccum);
+      const int sb = qi * 2 + (t & 1);
+      const uint32_t ts = lane_base + (uint32_t)(sb * kXKeys);
+      ok = x_wait(&s_full[sb], (uint32_t)(t >> 1) & 1u, kDevTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
       const int k0 = t * kXKeys;
       const bool diagonal = k0 + kXKeys - 1 > tile_limit;  // uniform: some row's limit falls in the tile
-      const float4* cs = sc + (t & 1) * kXBlocks;
+      const float4* cs = sc + (t & 3) * 4;
       uint32_t s[2][32];
-      // 64 raw scores of the tile, -inf where the row does not see the key
-      auto load_half = [&](int half) {
-        tmem_ld_32x32b_x32(ts + 64 * half, s[0]);
-        tmem_ld_32x32b_x32(ts + 64 * half + 32, s[1]);
-        tmem_ld_wait();
-        if (diagonal) {
-          const int seen = limit - k0 - 64 * half;
+      tmem_ld_32x32b_x32(ts, s[0]);
+      tmem_ld_32x32b_x32(ts + 32, s[1]);
+      tmem_ld_wait();
+      if (diagonal) {  // -inf where the row does not see the key
+        const int seen = limit - k0;
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i > seen) s[i >> 5][i & 31] = 0xff800000u;
-        }
-      };
+        for (int i = 0; i < kXKeys; ++i)
+          if (i > seen) s[i >> 5][i & 31] = 0xff800000u;
+      }
       float mt = -INFINITY;
-#pragma unroll 1
-      for (int half = 1; half >= 0; --half) {  // the lower half stays in registers
-        load_half(half);
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          const uint32_t* x = &s[jj >> 1][(jj & 1) * 16];
-          float mj = __uint_as_float(x[0]);
-#pragma unroll
-          for (int i = 1; i < 16; ++i) mj = fmaxf(mj, __uint_as_float(x[i]));
-          const float4 k = cs[4 * half + jj];
-          mt = fmaxf(mt, mj == -INFINITY ? -INFINITY : fmaf(mj, k.x * c, k.y));
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float mj = x_max16(&s[j >> 1][16 * (j & 1)]);
+        const float4 k = cs[j];
+        mt = fmaxf(mt, mj == -INFINITY ? -INFINITY : fmaf(mj, k.x * c, k.y));
       }
       float corr = 1.f;
       if (mt > m_used + 8.f) {                        // also true on the first tile
@@ -400,32 +551,36 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       }
       const float mu = m_used == -INFINITY ? 0.f : m_used;
       float sum = 0.f;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        if (half == 1) load_half(1);
-        uint32_t p[32];
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          const int j = 4 * half + jj;
-          const uint32_t* x = &s[jj >> 1][(jj & 1) * 16];
+      for (int q = 0; q < 2; ++q) {
+        uint32_t p[16];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const int j = 2 * q + jj;
+          const uint32_t* x = &s[q][16 * jj];
           const float4 k = cs[j];
           // a block that this row does not see must not reach it even as NaN
           const bool hidden = diagonal && k0 + 16 * j > limit;
           const float kc = hidden ? 1.f : k.x * c, off = hidden ? 0.f : k.y - mu;
-          float sj = 0.f;
+          float sa = 0.f, sb2 = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const float w0 = x_exp2(fmaf(__uint_as_float(x[i]), kc, off));
             const float w1 = x_exp2(fmaf(__uint_as_float(x[i + 1]), kc, off));
-            sj += w0 + w1;
+            sa += w0;
+            sb2 += w1;
             p[8 * jj + i / 2] = pack_f16x2(w0, w1);
           }
-          sum = hidden ? sum : fmaf(sj, k.z, sum);
+          sum = hidden ? sum : fmaf(sa + sb2, k.z, sum);
         }
-        tmem_st_32x32b_x32(ts + 32 * half, p);  // over columns of S that are in registers
+        x_tmem_st16(ts + 16 * q, p);                  // over S, which is in registers
       }
       l = l * corr + sum;
       if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+        // P V of t - 1 is in O (that of t - 2 is, or S(t) would not be)
+        ok = x_wait(&o_done[qi], (uint32_t)(t - 1) & 1u, kDevTimeoutAccum);
+        if (!ok) break;
+        tc_fence_after();
         uint32_t rr[32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -439,9 +594,9 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[qi]);
+      if (lane == 0) mbar_arrive(&p_full[sb]);
     }
-    if (ok) ok = x_wait(&o_done[qi], 0, kDevTimeoutAccum);
+    if (ok) ok = x_wait(&o_last[qi], 0, kDevTimeoutAccum);
     if (ok) {
       tc_fence_after();
       const float inv = 1.f / l;
@@ -469,7 +624,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 11) {
+  if (warp == kXIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
