@@ -15,14 +15,16 @@
 // row's chain softmax -> P V -> Q K^T -> softmax took 5,250 clocks per 128 keys, of
 // which the tensor core worked 2,050.
 //
-// Warp roles (14 warps of up to 128 registers):
+// Warp roles (16 warps of 128 registers; 14 has none):
 //   0-3, 4-7   softmax of query tile 0 / 1, one thread per row: S from TMEM, mask,
 //              weights back into TMEM over S (f16, the A operand of P V), O / l out.
-//   8-11       conversion of codes to f16, 16 at a time, into 128-byte swizzled K-major
+//   8, 15      issue PV(t), QK(t + 2) of query tile 0 / 1 (8 also owns TMEM).  S(t + 2)
+//              overwrites P(t): MMAs of one thread execute in order.
+//   9-11, 13   conversion of codes to f16, 16 at a time, into 128-byte swizzled K-major
 //              (K) / MN-major (V) panels, three stages each.
-//   12         TMEM owner; issues PV_i(t), QK_i(t + 2) for i = 0, 1 in turn.
-//              S_i(t + 2) overwrites P_i(t): MMAs of one thread execute in order.
-//   13         copies the paged blocks' codes (2 KB each, cp.async.bulk) into a ring.
+//   12         copies the paged blocks' codes (2 KB each, cp.async.bulk) into a ring.
+// (An issuing warp slows the others of its SM sub-partition, which warps w, w + 4, ...
+// share: no conversion warp sits beside the first, one beside the second.)
 // TMEM: S_i of tile t at 128 i + 64 (t & 1), O_i at 256 + 128 i.
 //
 // The running bound only moves when a tile exceeds it by more than 8, so weights
@@ -43,13 +45,18 @@ namespace muk {
 constexpr int kXD = 128;             // head_dim
 constexpr int kXRows = 128;          // rows of a query tile
 constexpr int kXKeys = 64;           // keys of a tile
-constexpr int kXThreads = 448;
-constexpr int kXConvert = 4;         // conversion warps, after the eight of the softmax
-constexpr int kXIssuer = 12;         // the warp that owns TMEM and issues the multiplies
-constexpr int kXLoader = 13;         // the warp that issues the copies of codes
-constexpr int kXStages = 3;          // converted K tiles, and V tiles
+constexpr int kXThreads = 512;
+constexpr int kXConvert = 4;         // conversion warps: 9, 10, 11 and 13
+constexpr int kXIssuer = 8;          // owns TMEM and issues the multiplies of query tile 0
+constexpr int kXIssuer1 = 15;        // issues those of query tile 1
+constexpr int kXLoader = 12;         // the warp that issues the copies of codes
+constexpr int kXStages = 3;          // converted steps: V(t) and K(t + 2)
 constexpr int kXRing = 3;            // steps (a V and a K tile) of codes on their way
 constexpr int kXItem = kXKeys * 128; // bytes of such a tile
+// Tiles of block constants: the loader is at most kXRing + kXStages + 1 tiles ahead of a
+// softmax warp.
+constexpr int kXConsts = 16;
+static_assert(kXConsts > kXRing + kXStages + 2, "block constants are overwritten in use");
 constexpr int kXQPanel = 128 * 128;  // [128 rows][64 f16], one swizzled panel of a query tile
 constexpr int kXPanel = kXKeys * 128;  // the same of a K or V tile
 
@@ -60,15 +67,15 @@ struct XLayout {
   static constexpr int kV = kK + kXStages * kStage;
   static constexpr int kRaw = kV + kXStages * kStage;
   static constexpr int kBar = kRaw + kXRing * 2 * kXItem;
-  static constexpr int kScale = kBar + 256;                  // [8 warps][2][8 blocks] float4
-  static constexpr int kRawScale = kScale + 8 * 2 * 8 * 16;  // [8 warps][8 blocks] (ks, vs)
-  static constexpr int kBytes = kRawScale + 8 * 64 + 1024;   // + alignment slack
+  static constexpr int kScale = kBar + 256;                  // [kXConsts tiles][4 blocks] float4
+  static constexpr int kBytes = kScale + kXConsts * 4 * 16 + 1024;  // + alignment slack
 };
 static_assert(XLayout::kBytes <= 232448, "prefill tile exceeds 227 KB of shared memory");
 
-// Bounded wait of a whole warp (about a second).  The polls are one loop in PTX: as
-// a C++ loop a wait on a barrier that was complete already took ~250 clocks.
-__device__ __forceinline__ bool x_wait(uint64_t* bar, uint32_t parity, int code) {
+// Bounded wait of a whole warp (about a second).  One try on a complete barrier is
+// ~110 clocks, so roles keep few barriers; the polls are one loop in PTX (as a C++ loop
+// with its checks inside, a wait took ~250).
+__device__ __noinline__ bool x_wait_long(uint32_t bar, uint32_t parity, int code) {
   for (int round = 0; round < 64; ++round) {
     uint32_t done;
     asm volatile(
@@ -86,13 +93,27 @@ __device__ __forceinline__ bool x_wait(uint64_t* bar, uint32_t parity, int code)
         "selp.u32 %0, 1, 0, p;\n"
         "}\n"
         : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
+        : "r"(bar), "r"(parity)
         : "memory");
     if (__all_sync(0xffffffffu, done != 0)) return true;
     if (*reinterpret_cast<volatile int*>(&g_device_error) != 0) break;
   }
   set_device_error(code);  // keeps an earlier code
   return false;
+}
+__device__ __forceinline__ bool x_wait(uint64_t* bar, uint32_t parity, int code) {
+  uint32_t done;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  if (__all_sync(0xffffffffu, done != 0)) return true;
+  return x_wait_long(smem_u32(bar), parity, code);
 }
 __device__ __forceinline__ uint32_t x_elect() {
   uint32_t r;
@@ -185,11 +206,9 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* basep = smem_raw + (base - raw);
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(basep + XLayout::kBar);
-  uint64_t* k_empty = k_full + kXStages;
-  uint64_t* v_full = k_empty + kXStages;
-  uint64_t* v_empty = v_full + kXStages;
-  uint64_t* s_full = v_empty + kXStages;  // [query tile][buffer] S complete
+  uint64_t* st_full = reinterpret_cast<uint64_t*>(basep + XLayout::kBar);  // [stage] step converted
+  uint64_t* st_empty = st_full + kXStages;                                 // [stage] and used
+  uint64_t* s_full = st_empty + kXStages; // [query tile][buffer] S complete
   uint64_t* p_full = s_full + 4;          // [query tile][buffer] weights written
   uint64_t* o_done = p_full + 4;          // [query tile] P V of a tile complete
   uint64_t* o_last = o_done + 2;          // [query tile] P V of the last tile complete
@@ -197,7 +216,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   uint64_t* raw_empty = raw_full + kXRing;
   uint64_t* q_full = raw_empty + kXRing;
   uint64_t* drain = q_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.x;
@@ -223,10 +242,8 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kXStages; ++i) {
-      mbar_init(&k_full[i], kXConvert);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], kXConvert);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&st_full[i], kXConvert);
+      mbar_init(&st_empty[i], 2);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -241,7 +258,8 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       mbar_init(&raw_empty[i], kXConvert);
     }
     mbar_init(q_full, 8);
-    mbar_init(drain, 1);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     fence_mbar_init();
   }
   if (warp == kXIssuer) {
@@ -253,69 +271,62 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == kXIssuer) {
-    // ---- MMA issuer ---------------------------------------------------------
+  if (warp == kXIssuer || warp == kXIssuer1) {
+    // ---- MMA issuers ---------------------------------------------------------
     const uint32_t lead = x_elect();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t dq = umma_desc_sw128(base + XLayout::kQ);
     const uint64_t dk = umma_desc_sw128(base + XLayout::kK);
     const uint64_t dv = umma_desc_sw128_mn(base + XLayout::kV, kXPanel, 1024);
-    // descriptors count addresses in 16-byte units
-    auto qk = [&](int i, int t) {  // S_i(t) = Q_i K_t^T
-      const uint64_t k0 = dk + (uint64_t)((t % kXStages) * (XLayout::kStage >> 4));
-      const uint32_t d = tm + (uint32_t)(i * 2 * kXKeys + (t & 1) * kXKeys);
+    const int qi = warp == kXIssuer ? 0 : 1;           // this warp's query tile
+    const uint64_t dqi = dq + (uint64_t)((qi * 2 * kXQPanel) >> 4);  // addresses in 16-byte units
+    const uint32_t s_at = tm + (uint32_t)(qi * 2 * kXKeys), o_at = tm + (uint32_t)(4 * kXKeys + qi * kXD);
+    auto qk = [&](int t, int sg) {  // S(t) = Q K_t^T
+      const uint64_t k0 = dk + (uint64_t)(sg * (XLayout::kStage >> 4));
+      const uint32_t d = s_at + (uint32_t)((t & 1) * kXKeys);
 #pragma unroll
       for (int k = 0; k < kXD / 16; ++k)
-        x_mma_ss(lead, d, dq + (uint64_t)((i * 2 * kXQPanel + (k >> 2) * kXQPanel + (k & 3) * 32) >> 4),
+        x_mma_ss(lead, d, dqi + (uint64_t)(((k >> 2) * kXQPanel + (k & 3) * 32) >> 4),
                  k0 + (uint64_t)(((k >> 2) * kXPanel + (k & 3) * 32) >> 4), x_idesc(false, kXKeys),
                  k > 0 ? 1u : 0u);
-      x_commit(lead, &s_full[i * 2 + (t & 1)]);
+      x_commit(lead, &s_full[qi * 2 + (t & 1)]);
     };
-    auto pv = [&](int i, int t) {  // O_i += P_i(t) V_t
-      const uint64_t v0 = dv + (uint64_t)((t % kXStages) * (XLayout::kStage >> 4));
-      const uint32_t p = tm + (uint32_t)(i * 2 * kXKeys + (t & 1) * kXKeys);
+    auto pv = [&](int t, int sg) {  // O += P(t) V_t
+      const uint64_t v0 = dv + (uint64_t)(sg * (XLayout::kStage >> 4));
+      const uint32_t p = s_at + (uint32_t)((t & 1) * kXKeys);
 #pragma unroll
       for (int k = 0; k < kXKeys / 16; ++k)
-        x_mma_ts(lead, tm + (uint32_t)(4 * kXKeys + i * kXD), p + (uint32_t)(k * 8),
-                 v0 + (uint64_t)((k * 16 * 128) >> 4), x_idesc(true, kXD), (t > 0 || k > 0) ? 1u : 0u);
+        x_mma_ts(lead, o_at, p + (uint32_t)(k * 8), v0 + (uint64_t)((k * 16 * 128) >> 4),
+                 x_idesc(true, kXD), (t > 0 || k > 0) ? 1u : 0u);
       // a barrier of its own for the last one: its reader may be two tiles ahead of the
       // multiplies there, which the phase of o_done cannot tell
-      x_commit(lead, t + 1 < nt ? &o_done[i] : &o_last[i]);
+      x_commit(lead, t + 1 < nt ? &o_done[qi] : &o_last[qi]);
     };
+    // Step t = -2 .. nt - 1 uses V(t) and K(t + 2) of stage (t + 2) % kXStages.
     bool ok = x_wait(q_full, 0, kDevTimeoutFull);
-    for (int t = 0; ok && t < 2 && t < nt; ++t) {
-      ok = x_wait(&k_full[t], 0, kDevTimeoutFull);
+    int sg = 0;
+    uint32_t ph = 0;
+    for (int t = -2; ok && t < nt; ++t) {
+      ok = x_wait(&st_full[sg], ph, kDevTimeoutFull);
+      if (ok && t >= 0) ok = x_wait(&p_full[qi * 2 + (t & 1)], (uint32_t)(t >> 1) & 1u, kDevTimeoutFull);
       if (!ok) break;
       tc_fence_after();
-      qk(0, t);
-      qk(1, t);
-      x_commit(lead, &k_empty[t]);
-    }
-    for (int t = 0; ok && t < nt; ++t) {
-      const int n = t + 2;
-      const bool more = n < nt;
-      if (!x_wait(&v_full[t % kXStages], (uint32_t)(t / kXStages) & 1u, kDevTimeoutFull)) break;
-      if (more && !x_wait(&k_full[n % kXStages], (uint32_t)(n / kXStages) & 1u, kDevTimeoutFull)) break;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ok = x_wait(&p_full[i * 2 + (t & 1)], (uint32_t)(t >> 1) & 1u, kDevTimeoutFull);
-        if (!ok) break;
-        tc_fence_after();
-        pv(i, t);
-        if (i == 1) x_commit(lead, &v_empty[t % kXStages]);
-        if (more) qk(i, n);
-        if (i == 1 && more) x_commit(lead, &k_empty[n % kXStages]);
-      }
+      if (t >= 0) pv(t, sg);
+      if (t + 2 < nt) qk(t + 2, sg);
+      x_commit(lead, &st_empty[sg]);
+      if (++sg == kXStages) sg = 0, ph ^= 1;
     }
     // every MMA this warp issued has finished before TMEM is freed, also when a
     // wait above gave up
-    x_commit(lead, drain);
-    x_wait(drain, 0, kDevTimeoutAccum);
+    x_commit(lead, &drain[qi]);
+    x_wait(&drain[qi], 0, kDevTimeoutAccum);
   } else if (warp == kXLoader) {
     // ---- loads of codes -------------------------------------------------------
     // Step t brings V(t) and K(t + 2), which the multiplies of one step need (steps -2
     // and -1: K alone): lanes 0-3 a block of V each, 4-7 one of K, 2 KB a copy.  Blocks
-    // behind the last key are left out (their rows become zero when converted).
+    // behind the last key are left out (their rows become zero when converted).  Lanes 0-3
+    // also leave the constants of their block of tile t (ks, log2 vs, 1 / vs) for the
+    // softmax warps, whose S(t) comes after the conversion of these codes.
     const bool mine_k = lane >= 4;
     const uint8_t* src = (mine_k ? a.k_cache : a.v_cache) + (int64_t)kvh * (kKvBlock * kXD);
     const int64_t blk_bytes = (int64_t)a.num_kv_heads * (kKvBlock * kXD);
@@ -326,19 +337,33 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     };
     auto id_of = [&](int t) {
       const int blk = block_of(t);
-      int id = blk >= 0 ? __ldg(bt + blk) : 0;
-      if (id < 0 || id >= a.num_blocks) {
-        set_device_error(kDevBadIndex);
-        id = 0;
-      }
-      return id;
+      return blk >= 0 ? __ldg(bt + blk) : 0;
     };
+    auto scales_of = [&](int t, int i) {             // of this lane's block of tile t (lanes 0-3)
+      const int64_t at = (int64_t)(i >= 0 && i < a.num_blocks ? i : 0) * a.num_kv_heads + kvh;
+      return lane < 4 && block_of(t) >= 0 ? make_float2(__ldg(a.k_scale + at), __ldg(a.v_scale + at))
+                                          : make_float2(1.f, 1.f);
+    };
+    float4* consts = reinterpret_cast<float4*>(basep + XLayout::kScale);
     int id = id_of(-2), id_next = id_of(-1), slot = 0, issued = 0;
+    float2 scales = make_float2(1.f, 1.f);           // of tile t
     uint32_t ph = 1;
     for (int t = -2; t < nt; ++t) {
       if (!x_wait(raw_empty + slot, ph, kDevTimeoutEmpty)) break;
       const bool have = block_of(t) >= 0;
       const int blocks = __popc(__ballot_sync(0xffffffffu, have));
+      if (id < 0 || id >= a.num_blocks) {
+        set_device_error(kDevBadIndex);
+        id = 0;
+      }
+      if (t >= 0 && lane < 4) {
+        const float ks = clamp_scale(scales.x), vs = clamp_scale(scales.y);
+        float lv, iv;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(vs));  // exact for powers of two
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(iv) : "f"(vs));
+        consts[(t % kXConsts) * 4 + lane] = make_float4(ks, lv, iv, 0.f);
+      }
+      __syncwarp();
       if (lane == 0) mbar_arrive_expect_tx(raw_full + slot, (uint32_t)(blocks * 2048));
       __syncwarp();
       if (have)
@@ -350,18 +375,19 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       ++issued;
       id = id_next;
       id_next = id_of(t + 2);
+      scales = scales_of(t + 1, id);
       if (++slot == kXRing) slot = 0, ph ^= 1;
     }
     // No copy may still be on its way when the CTA ends, also where the others gave up:
     // the last copies into each slot have arrived.
     for (int m = max(issued - kXRing, 0); m < issued; ++m)
       x_wait(raw_full + m % kXRing, (uint32_t)(m / kXRing) & 1u, kDevTimeoutFull);
-  } else if (warp >= 8) {
+  } else if (warp >= 8 && warp != 14) {
     // ---- conversion -----------------------------------------------------------
     // Warp w takes rows 4w .. 4w + 3 of every block (512 contiguous bytes), a lane one
     // 16-code chunk of them.  Eight neighbouring lanes cover two rows of one panel,
     // which the swizzle puts into all 32 banks.
-    const int w = warp - 8, row = 4 * w + (lane >> 4) * 2 + ((lane >> 2) & 1);
+    const int w = warp == 13 ? 3 : warp - 9, row = 4 * w + (lane >> 4) * 2 + ((lane >> 2) & 1);
     const int c = (lane & 3) + ((lane >> 3) & 1) * 4;
     constexpr int kBpt = kXKeys / kKvBlock;          // blocks of a tile
     const uint32_t ring = base + (uint32_t)(XLayout::kRaw + row * kXD + c * 16);
@@ -397,36 +423,28 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
                      "r"(x[6]), "r"(x[7]) : "memory");
       }
     };
-    int slot = 0, sg_v = 0, sg_k = 0;
-    uint32_t ph_r = 0;                               // parity of the ring's "full" barriers
-    uint32_t ph_v = 1, ph_k = 1;                     // parities of the stages' "empty" barriers
-    for (int t = -2; t < nt; ++t) {
+    int slot = 0, sg = 0;
+    uint32_t ph_r = 0, ph = 1;                       // parities: ring "full", stage "empty"
+    for (int t = -2; t < nt; ++t) {                  // step t: V(t) and K(t + 2)
       const bool has_v = t >= 0, has_k = t + 2 < nt;
       uint4 vv[kBpt], vk[kBpt];
       if (!x_wait(raw_full + slot, ph_r, kDevTimeoutFull)) break;
       const uint32_t src = ring + (uint32_t)(slot * 2 * kXItem);
       if (has_v) read(vv, src);
       if (has_k) read(vk, src + kXItem);
-      if (has_v) {
-        if (!x_wait(v_empty + sg_v, ph_v, kDevTimeoutEmpty)) break;
-        convert(vv, t, (uint32_t)(XLayout::kV + sg_v * XLayout::kStage));
-      }
-      if (has_k) {
-        if (!x_wait(k_empty + sg_k, ph_k, kDevTimeoutEmpty)) break;
-        convert(vk, t + 2, (uint32_t)(XLayout::kK + sg_k * XLayout::kStage));
-      }
+      if (!x_wait(st_empty + sg, ph, kDevTimeoutEmpty)) break;
+      if (has_v) convert(vv, t, (uint32_t)(XLayout::kV + sg * XLayout::kStage));
+      if (has_k) convert(vk, t + 2, (uint32_t)(XLayout::kK + sg * XLayout::kStage));
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (has_v) mbar_arrive(v_full + sg_v);
-        if (has_k) mbar_arrive(k_full + sg_k);
+        mbar_arrive(st_full + sg);
         mbar_arrive(raw_empty + slot);
       }
-      if (has_v && ++sg_v == kXStages) sg_v = 0, ph_v ^= 1;
-      if (has_k && ++sg_k == kXStages) sg_k = 0, ph_k ^= 1;
+      if (++sg == kXStages) sg = 0, ph ^= 1;
       if (++slot == kXRing) slot = 0, ph_r ^= 1;
     }
-  } else {
+  } else if (warp < 8) {
     // ---- softmax / epilogue: one thread per query row --------------------------
     const int qi = warp >> 2;                        // query tile
     const int r = (warp & 3) * 32 + lane;            // row = TMEM lane
@@ -473,52 +491,10 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    // Block constants (ks, log2 vs, 1 / vs) of two tiles at a time, in the warp's own
-    // buffers: lanes 0-7 read a block's id two pairs ahead and copy its scales one
-    // pair ahead (cp.async: a load into a register would be waited for together with
-    // every other load in flight).
-    float4* sc = reinterpret_cast<float4*>(basep + XLayout::kScale) + warp * 16;
-    const uint32_t raw_sc = base + (uint32_t)(XLayout::kRawScale + warp * 64 + (lane & 7) * 8);
-    auto get_id = [&](int u) {
-      const int blk = u * 8 + (lane & 7);
-      const int id = blk < nblk ? __ldg(bt + blk) : 0;
-      return id >= 0 && id < a.num_blocks ? id : 0;  // bad ids are latched by the converters
-    };
-    auto copy_scales = [&](int id) {
-      const int64_t at = (int64_t)id * a.num_kv_heads + kvh;
-      if (lane < 8) {
-        cp_async_4(raw_sc, a.k_scale + at);
-        cp_async_4(raw_sc + 4, a.v_scale + at);
-      }
-      cp_async_commit();
-    };
-    auto put = [&](int u) {
-      cp_async_wait<0>();
-      if (lane < 8) {
-        // blocks behind the last key are hidden from every row, whatever stands here
-        const float ks = clamp_scale(ld_shared_f32(raw_sc)), vs = clamp_scale(ld_shared_f32(raw_sc + 4));
-        float lv, iv;
-        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(vs));   // exact for powers of two
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(iv) : "f"(vs));
-        sc[(u & 1) * 8 + lane] = make_float4(ks, lv, iv, 0.f);
-      }
-    };
-    const int nu = (nt + 1) >> 1;
-    copy_scales(get_id(0));
-    put(0);
-    if (nu > 1) copy_scales(get_id(1));
-    int id_next = nu > 2 ? get_id(2) : 0;
-    __syncwarp();
-
+    const float4* consts = reinterpret_cast<const float4*>(basep + XLayout::kScale);
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < nt; ++t) {
-      if ((t & 1) == 0 && (t >> 1) + 1 < nu) {
-        const int u = t >> 1;
-        put(u + 1);
-        if (u + 2 < nu) copy_scales(id_next);
-        if (u + 3 < nu) id_next = get_id(u + 3);
-      }
       const int sb = qi * 2 + (t & 1);
       const uint32_t ts = lane_base + (uint32_t)(sb * kXKeys);
       ok = x_wait(&s_full[sb], (uint32_t)(t >> 1) & 1u, kDevTimeoutAccum);
@@ -526,7 +502,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       tc_fence_after();
       const int k0 = t * kXKeys;
       const bool diagonal = k0 + kXKeys - 1 > tile_limit;  // uniform: some row's limit falls in the tile
-      const float4* cs = sc + (t & 3) * 4;
+      const float4* cs = consts + (t % kXConsts) * 4;
       uint32_t s[2][32];
       tmem_ld_32x32b_x32(ts, s[0]);
       tmem_ld_32x32b_x32(ts + 32, s[1]);
