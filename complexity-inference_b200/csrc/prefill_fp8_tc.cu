@@ -52,6 +52,7 @@ constexpr int kXIssuer1 = 15;        // issues those of query tile 1
 constexpr int kXLoader = 12;         // the warp that issues the copies of codes
 constexpr int kXStages = 3;          // converted steps: V(t) and K(t + 2)
 constexpr int kXRing = 3;            // steps (a V and a K tile) of codes on their way
+constexpr int kXFmaMask = 2;         // of 16 weights those i + 1 with (i & mask) == mask, i even: a quarter
 constexpr int kXItem = kXKeys * 128; // bytes of such a tile
 // Tiles of block constants: the loader is at most kXRing + kXStages + 1 tiles ahead of a
 // softmax warp.
@@ -131,6 +132,20 @@ __device__ __forceinline__ float x_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^x on the FMA pipe, for a part of the weights (MUFU takes 8 clocks a warp, and was
+// busy 1,024 of a tile's ~2,200): 2^n * p(f), n = round(x) from the bits of x + 1.5 * 2^23,
+// f = x - n in [-1/2, 1/2], p the degree-4 minimax polynomial of 2^f (relative error
+// 2^-18.5, fitted for this; f16 keeps 2^-11).  Below 2^-126 it returns 2^-126.
+__device__ __forceinline__ float x_exp2_fma(float x) {
+  x = fmaxf(x, -126.f);
+  const float z = x + 12582912.f;
+  const float f = x - (z - 12582912.f);
+  float p = fmaf(f, 0.0095701013f, 0.0559178628f);
+  p = fmaf(p, f, 0.2402474433f);
+  p = fmaf(p, f, 0.6931217909f);
+  p = fmaf(p, f, 0.9999992847f);
+  return __int_as_float(__float_as_int(p) + (__float_as_int(z) << 23));
 }
 __device__ __forceinline__ float x_max3(float a, float b, float c) {
   float y;
@@ -542,7 +557,8 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const float w0 = x_exp2(fmaf(__uint_as_float(x[i]), kc, off));
-            const float w1 = x_exp2(fmaf(__uint_as_float(x[i + 1]), kc, off));
+            const float y1 = fmaf(__uint_as_float(x[i + 1]), kc, off);
+            const float w1 = (i & kXFmaMask) == kXFmaMask ? x_exp2_fma(y1) : x_exp2(y1);
             sa += w0;
             sb2 += w1;
             p[8 * jj + i / 2] = pack_f16x2(w0, w1);
