@@ -16,10 +16,13 @@
 // NaN, as they would a bf16 cache holding that value.
 //
 // Work.  A run = neighbouring batch rows that land in one block (one sequence's
-// new tokens: a single row in a decode step, up to 16 in a prefill).  One warp
-// owns one (run, K or V head): all its rows stay in registers between the
-// maximum and the rounding, so q|k|v is read once.  q rows are rotated by
-// further CTAs of the same launch.
+// new tokens: a single row in a decode step, up to 16 in a prefill).  A CTA owns
+// the runs that start in a window of rows, for a few K / V heads; a head's 16
+// rows are spread over two or four warps, 16 elements a thread, which stay in
+// registers between the maximum (exchanged through shared memory) and the
+// rounding: q|k|v is read once.  (A whole head in one warp, 64 elements a thread,
+// took 242 registers and left one CTA on an SM: 141 us for 8k rows.)  q rows are
+// rotated by further CTAs of the same launch.
 //
 // The rotation is a*c - b*s with every product rounded (no fused multiply-add)
 // and the QK-norm factor is formed in f64: next to a rounding border of e4m3 the
@@ -51,12 +54,16 @@ struct KvFp8Args {
   float* k_scale;
   float* v_scale;
   int num_blocks;
-  int window;      // batch rows per K/V CTA: the runs that start in them are its own
-  int kv_ctas;     // leading CTAs: windows x head groups
-  int head_groups; // K/V heads are spread over this many CTAs per window
+  int groups;         // groups of K / V heads that a window CTA works on together
+  int groups_per_cta, group_ctas;
+  int kv_ctas;        // leading CTAs: windows of rows x group_ctas
+  int single_ctas;    // next: rows that are alone in their block; 0: the windows take them too
+  int q_tokens;       // the others: q of this many rows each
 };
 
+constexpr int kWindow = 16;          // batch rows of a window CTA: the runs that start in them are its own
 constexpr int kAppendThreads = 256;
+constexpr int kAppendCtas = 3;      // resident per SM: 48 registers; 3 (79 registers) was 80 us for 8k rows, 5 is 61
 
 // 8 + 8 elements of a head: i0 .. i0+7 of the first half and their partners.
 __device__ __forceinline__ void unpack16(const uint4& lo, const uint4& hi, float (&x)[16]) {
@@ -71,30 +78,49 @@ __device__ __forceinline__ void unpack16(const uint4& lo, const uint4& hi, float
   }
 }
 
-// RMSNorm over the head, whose elements lie in D/16 neighbouring lanes.
+// RMSNorm over the head, whose elements (bf16 numbers) lie in D/16 neighbouring
+// lanes (all lanes of the warp take part, `on` lanes change).  The sum of squares is f64; |x| becomes an f64 by its bits, exponent
+// rebiased (a conversion instruction runs at an eighth of the rate), which leaves
+// subnormals off by less than 2^-126.  1 / sqrt is f32's estimate and one Newton
+// step in f64 (2^-43), rounded to f32.
 template <int D>
-__device__ __forceinline__ void head_norm(float (&x)[16], const float* w, int i0, double eps) {
+__device__ __forceinline__ void head_norm(float (&x)[16], const float* w, int i0, double eps, bool on) {
   double ss = 0.0;
 #pragma unroll
-  for (int u = 0; u < 16; ++u) ss += (double)x[u] * (double)x[u];
+  for (int u = 0; u < 16; ++u) {
+    const double v =
+        __hiloint2double((int)(((__float_as_uint(x[u]) & 0x7fffffffu) >> 3) + (896u << 20)), 0);
+    ss = fma(v, v, ss);
+  }
 #pragma unroll
   for (int m = D / 32; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-  const float inv = (float)(1.0 / sqrt(ss / (double)D + eps));
+  const double m = ss * (1.0 / D) + eps;
+  const double y = (double)rsqrtf((float)m);
+  float inv = (float)(y * (1.5 - 0.5 * m * y * y));
+  if (!(m > 1e-37 && m < 1e37)) inv = (float)(1.0 / sqrt(m));        // m or y beyond f32: the long way
+  if (ss >= 0x1p256) inv = __int_as_float(0x7fffffff);  // infinities and NaN among the elements
+  if (on) {
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    x[u] = __fmul_rn(w[i0 + u], __fmul_rn(x[u], inv));
-    x[8 + u] = __fmul_rn(w[D / 2 + i0 + u], __fmul_rn(x[8 + u], inv));
+    for (int u = 0; u < 8; ++u) {
+      x[u] = __fmul_rn(w[i0 + u], __fmul_rn(x[u], inv));
+      x[8 + u] = __fmul_rn(w[D / 2 + i0 + u], __fmul_rn(x[8 + u], inv));
+    }
   }
 }
 
+// cos and sin of 8 neighbouring pairs at a position.
+struct Rope8 {
+  float4 c0, c1, s0, s1;
+};
 template <int D>
-__device__ __forceinline__ void rotate16(float (&x)[16], const float* rope_cos,
-                                         const float* rope_sin, int pos, int i0) {
-  const float4* cs = reinterpret_cast<const float4*>(rope_cos + (int64_t)pos * (D / 2) + i0);
-  const float4* sn = reinterpret_cast<const float4*>(rope_sin + (int64_t)pos * (D / 2) + i0);
-  const float4 c0 = __ldg(cs), c1 = __ldg(cs + 1), s0 = __ldg(sn), s1 = __ldg(sn + 1);
-  const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-  const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+__device__ __forceinline__ Rope8 load_rope(const KvFp8Args& a, int pos, int i0) {
+  const float4* cs = reinterpret_cast<const float4*>(a.rope_cos + (int64_t)pos * (D / 2) + i0);
+  const float4* sn = reinterpret_cast<const float4*>(a.rope_sin + (int64_t)pos * (D / 2) + i0);
+  return {__ldg(cs), __ldg(cs + 1), __ldg(sn), __ldg(sn + 1)};
+}
+__device__ __forceinline__ void rotate16(float (&x)[16], const Rope8& r) {
+  const float c[8] = {r.c0.x, r.c0.y, r.c0.z, r.c0.w, r.c1.x, r.c1.y, r.c1.z, r.c1.w};
+  const float s[8] = {r.s0.x, r.s0.y, r.s0.z, r.s0.w, r.s1.x, r.s1.y, r.s1.z, r.s1.w};
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const float a = x[u], b = x[8 + u];
@@ -116,189 +142,270 @@ __device__ __forceinline__ uint4 rescale16(uint4 v, float ratio) {
   return v;
 }
 
-// One warp: up to 16 rows t .. t+rows-1, all of one block, of K or V head h.
+// The block's new exponent and what its older codes are multiplied by, from the bits of
+// the new rows' largest |x| (top), its old scale and whether it starts anew; `bad`: the
+// scale becomes NaN.
+struct NewScale {
+  int e;
+  float ratio;
+  bool bad;
+};
+__device__ __forceinline__ NewScale new_scale(uint32_t top, float old, bool fresh) {
+  NewScale n;
+  // as integers, infinities and NaN come out above every finite value
+  n.bad = top >= 0x7f800000u || (!fresh && old != old);
+  n.e = n.bad ? 0 : scale_exponent(top);
+  n.ratio = 1.f;
+  if (!fresh && !n.bad) {
+    // exponent of the smallest power of two that is not below the old scale
+    const uint32_t ob = old > 0.f ? __float_as_uint(old) : 0u;
+    const int eo = (int)(ob >> 23) - 127 + ((ob & 0x7fffffu) != 0 ? 1 : 0);
+    n.e = max(n.e, min(max(eo, kScaleExpMin), kScaleExpMax));
+    n.ratio = old > 0.f ? old * pow2i(-n.e) : 0.f;
+  }
+  return n;
+}
+__device__ __forceinline__ float scale_value(const NewScale& n) {
+  return n.bad ? __int_as_float(0x7fffffff) : pow2i(n.e);
+}
+// A lane's 8 + 8 elements as codes; the scale says NaN where it has to, no code does.
+template <int D>
+__device__ __forceinline__ void store_row(uint8_t* row, int i0, const float (&x)[16], const NewScale& n) {
+  const float inv = pow2i(-n.e);
+  uint2 a8, b8;
+  a8.x = f32x4_to_e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  a8.y = f32x4_to_e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+  b8.x = f32x4_to_e4m3x4(x[8] * inv, x[9] * inv, x[10] * inv, x[11] * inv);
+  b8.y = f32x4_to_e4m3x4(x[12] * inv, x[13] * inv, x[14] * inv, x[15] * inv);
+  if (n.bad) a8 = b8 = make_uint2(0u, 0u);
+  *reinterpret_cast<uint2*>(row + i0) = a8;
+  *reinterpret_cast<uint2*>(row + D / 2 + i0) = b8;
+}
+__device__ __forceinline__ uint32_t top_bits(const float (&x)[16]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int u = 0; u < 16; ++u) top = max(top, __float_as_uint(x[u]) & 0x7fffffffu);
+  return top;
+}
+__device__ __forceinline__ int block_at(const KvFp8Args& a, int t) {
+  const int s = t >= 0 && t < a.num_tokens ? a.slots[t] : -1;
+  return s < 0 ? -1 : s / kKvBlock;
+}
+
+// A row that is alone in its block in this call (decode): the D / 16 lanes of one
+// (row, K or V head) do it by themselves.  All lanes of the warp take part.
+template <int D>
+__device__ __forceinline__ void append_single(const KvFp8Args& a, int64_t item) {
+  constexpr int kLanes = D / 16;
+  const int lane = threadIdx.x & 31, c = lane % kLanes, i0 = c * 8;
+  const int heads = 2 * a.num_kv_heads;
+  const bool in = item < (int64_t)a.num_tokens * heads;
+  const int t = in ? (int)(item / heads) : 0, j = in ? (int)(item - (int64_t)t * heads) : 0;
+  const bool is_k = j < a.num_kv_heads;
+  const int h = is_k ? j : j - a.num_kv_heads;
+  const int slot = a.slots[t], blk = slot < 0 ? -1 : slot / kKvBlock;
+  bool mine = in && blk >= 0 && block_at(a, t - 1) != blk && block_at(a, t + 1) != blk;
+  int pos = a.positions[t];
+  if (mine && (blk >= a.num_blocks || (is_k && (pos < 0 || pos >= a.max_pos)))) {
+    set_device_error(kDevBadIndex);
+    mine = false;
+  }
+  if (!mine || !is_k) pos = 0;
+  const int off = mine ? slot - blk * kKvBlock : 0;
+  const int64_t tile = (int64_t)(mine ? blk : 0) * a.num_kv_heads + h;
+  uint8_t* dst = (is_k ? a.k_cache : a.v_cache) + tile * (kKvBlock * D);
+  float* sc = (is_k ? a.k_scale : a.v_scale) + tile;
+  const bool fresh = off == 0;
+  const float old = mine ? *sc : 0.f;
+  const __nv_bfloat16* row = a.qkv + (int64_t)t * a.qkv_stride + (int64_t)(a.num_q_heads + j) * D;
+  const uint4 lo = *reinterpret_cast<const uint4*>(row + i0);
+  const uint4 hi = *reinterpret_cast<const uint4*>(row + D / 2 + i0);
+  float x[16];
+  unpack16(lo, hi, x);
+  if (a.k_norm_w != nullptr) head_norm<D>(x, a.k_norm_w, i0, a.qk_eps, is_k);
+  if (is_k) rotate16(x, load_rope<D>(a, pos, i0));
+  uint32_t top = top_bits(x);
+#pragma unroll
+  for (int m = kLanes / 2; m > 0; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+  const NewScale n = new_scale(top, old, fresh);
+  if (!mine) return;
+  if (n.ratio != 1.f) {  // the block's other rows move to the new scale
+#pragma unroll 4
+    for (int r = 0; r < kKvBlock; ++r) {
+      uint4* q = reinterpret_cast<uint4*>(dst + r * D) + c;
+      if (r != off) *q = rescale16(*q, n.ratio);
+    }
+  }
+  store_row<D>(dst + off * D, i0, x, n);
+  if (c == 0) *sc = scale_value(n);
+}
+
+// Up to 16 rows t .. t + rows - 1, all of block blk, of the K and V heads of groups g0 ..
+// g1 - 1 (kHeads neighbouring heads, K first, are a group): a warp has kPer rows of a
+// head, its lanes 16 elements each.  Every warp of the CTA calls it (one barrier a
+// group); the next group's rows are loaded while this one's are worked on.
 template <int D>
 __device__ __forceinline__ void append_rows(const KvFp8Args& a, int t, int rows, int blk, int slot,
-                                            bool is_k, int h) {
+                                            int g0, int g1, uint32_t (*red)[kAppendThreads / 32]) {
   constexpr int kLanes = D / 16;           // lanes of a row
-  constexpr int kPer = 32 / kLanes;        // rows at a time
-  constexpr int kPass = kKvBlock / kPer;
-  const int lane = threadIdx.x & 31;
-  const int c = lane % kLanes, sub = lane / kLanes, i0 = c * 8;
+  constexpr int kPer = 32 / kLanes;        // rows of a warp
+  constexpr int kWph = kKvBlock / kPer;    // warps of a head
+  constexpr int kHeads = kAppendThreads / 32 / kWph;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wq = warp % kWph;
+  const int c = lane % kLanes, i0 = c * 8, r = wq * kPer + lane / kLanes;
   // lane i holds row i's place; of rows naming one slot the last one counts
   const int off = slot - blk * kKvBlock;
   const uint32_t same = __match_any_sync(0xffffffffu, lane < rows ? off : 64 + lane);
-  bool valid = lane < rows && (31 - __clz(same)) == lane;
+  const bool valid = lane < rows && (31 - __clz(same)) == lane;
   int pos = lane < rows ? a.positions[t + lane] : 0;
-  if (is_k && lane < rows && (pos < 0 || pos >= a.max_pos)) {
+  const bool pos_ok = pos >= 0 && pos < a.max_pos;
+  if (lane < rows && !pos_ok) {
     set_device_error(kDevBadIndex);
-    valid = false;
     pos = 0;
   }
-  const uint32_t vmask = __ballot_sync(0xffffffffu, valid);
-  const uint32_t omask = __reduce_or_sync(0xffffffffu, valid ? 1u << off : 0u);
-  if (vmask == 0) return;
-
-  const __nv_bfloat16* src = a.qkv + (int64_t)t * a.qkv_stride +
-                             (int64_t)(a.num_q_heads + (is_k ? h : a.num_kv_heads + h)) * D;
-  const int64_t tile = (int64_t)blk * a.num_kv_heads + h;
-  uint8_t* dst = (is_k ? a.k_cache : a.v_cache) + tile * (kKvBlock * D);
-  float* sc = (is_k ? a.k_scale : a.v_scale) + tile;
-  const bool fresh = (omask & 1u) != 0;
-  const float old = fresh ? 0.f : *sc;
-
-  uint4 lo[kPass], hi[kPass];
-#pragma unroll
-  for (int j = 0; j < kPass; ++j) {
-    const int r = j * kPer + sub;
-    lo[j] = hi[j] = make_uint4(0u, 0u, 0u, 0u);
-    if ((vmask >> r) & 1u) {
-      const __nv_bfloat16* row = src + (int64_t)r * a.qkv_stride;
-      lo[j] = *reinterpret_cast<const uint4*>(row + i0);
-      hi[j] = *reinterpret_cast<const uint4*>(row + D / 2 + i0);
+  // of K rows those with a position, of V rows all
+  const uint32_t vk = __ballot_sync(0xffffffffu, valid && pos_ok), vv = __ballot_sync(0xffffffffu, valid);
+  const uint32_t ok = __reduce_or_sync(0xffffffffu, valid && pos_ok ? 1u << off : 0u);
+  const uint32_t ov = __reduce_or_sync(0xffffffffu, valid ? 1u << off : 0u);
+  const int o = __shfl_sync(0xffffffffu, off, r), p = __shfl_sync(0xffffffffu, pos, r);
+  const Rope8 rope = load_rope<D>(a, p, i0);
+  const __nv_bfloat16* row = a.qkv + (int64_t)(t + (r < rows ? r : 0)) * a.qkv_stride +
+                             (int64_t)a.num_q_heads * D + i0;
+  uint4 lo, hi;
+  auto load = [&](int g) {
+    const int j = g * kHeads + warp / kWph;
+    lo = hi = make_uint4(0u, 0u, 0u, 0u);
+    if (j < 2 * a.num_kv_heads && r < rows) {
+      lo = *reinterpret_cast<const uint4*>(row + (int64_t)j * D);
+      hi = *reinterpret_cast<const uint4*>(row + (int64_t)j * D + D / 2);
     }
-  }
-  float x[kPass][16];
-  uint32_t top = 0;
+  };
+  load(g0);
+  for (int g = g0; g < g1; ++g) {
+    const int j = g * kHeads + warp / kWph;
+    const bool live = j < 2 * a.num_kv_heads, is_k = j < a.num_kv_heads;
+    const int h = !live ? 0 : (is_k ? j : j - a.num_kv_heads);
+    const uint32_t vmask = !live ? 0u : (is_k ? vk : vv), omask = is_k ? ok : ov;
+    const bool mine = ((vmask >> r) & 1u) != 0, fresh = (omask & 1u) != 0;
+    const int64_t tile = (int64_t)blk * a.num_kv_heads + h;
+    uint8_t* dst = (is_k ? a.k_cache : a.v_cache) + tile * (kKvBlock * D);
+    float* sc = (is_k ? a.k_scale : a.v_scale) + tile;
+    const float old = fresh || !live ? 0.f : *sc;
+    float x[16];
+    unpack16(lo, hi, x);
+    if (g + 1 < g1) load(g + 1);
+    if (a.k_norm_w != nullptr) head_norm<D>(x, a.k_norm_w, i0, a.qk_eps, is_k);
+    if (is_k) rotate16(x, rope);
+    uint32_t top = __reduce_max_sync(0xffffffffu, mine ? top_bits(x) : 0u);
+    if (lane == 0) red[g & 1][warp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kPass; ++j) {
-    if (j * kPer < rows) {  // uniform
-      unpack16(lo[j], hi[j], x[j]);
-      if (is_k) {
-        if (a.k_norm_w != nullptr) head_norm<D>(x[j], a.k_norm_w, i0, a.qk_eps);
-        const int p = __shfl_sync(0xffffffffu, pos, j * kPer + sub);
-        rotate16<D>(x[j], a.rope_cos, a.rope_sin, p, i0);
-      }
-#pragma unroll
-      for (int u = 0; u < 16; ++u) top = max(top, __float_as_uint(x[j][u]) & 0x7fffffffu);
+    for (int w = 0; w < kWph; ++w) top = max(top, red[g & 1][warp - wq + w]);
+    if (vmask == 0) continue;
+    const NewScale n = new_scale(top, old, fresh);
+    // the block's other rows move to the new scale; a lane's share is chunk c of row r
+    if (n.ratio != 1.f && ((omask >> r) & 1u) == 0) {
+      uint4* q = reinterpret_cast<uint4*>(dst + r * D) + c;
+      *q = rescale16(*q, n.ratio);
     }
+    if (mine) store_row<D>(dst + o * D, i0, x, n);
+    // every warp of the head has read the old scale: they met at the barrier
+    if (lane == 0 && wq == 0) *sc = scale_value(n);
   }
-  // as integers, infinities and NaN come out above every finite value
-  top = __reduce_max_sync(0xffffffffu, top);
-  const bool bad = top >= 0x7f800000u || old != old;
-  int e = bad ? 0 : scale_exponent(top);
-  float ratio = 1.f;
-  if (!fresh && !bad) {
-    // exponent of the smallest power of two that is not below the old scale
-    const uint32_t ob = old > 0.f ? __float_as_uint(old) : 0u;
-    int eo = (int)(ob >> 23) - 127 + ((ob & 0x7fffffu) != 0 ? 1 : 0);
-    eo = min(max(eo, kScaleExpMin), kScaleExpMax);
-    e = max(e, eo);
-    ratio = old > 0.f ? old * pow2i(-e) : 0.f;
-  }
-  if (!fresh && !bad && ratio != 1.f) {  // the block's other rows move to the new scale
-    constexpr int kUnits = kKvBlock * D / 16 / 32;
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int unit = i * 32 + lane, row = unit / (D / 16);
-      if (((omask >> row) & 1u) == 0) {
-        uint4* p = reinterpret_cast<uint4*>(dst) + unit;
-        *p = rescale16(*p, ratio);
-      }
-    }
-  }
-  const float inv = pow2i(-e);
-#pragma unroll
-  for (int j = 0; j < kPass; ++j) {
-    const int r = j * kPer + sub;
-    const int o = __shfl_sync(0xffffffffu, off, r);
-    if ((vmask >> r) & 1u) {
-      uint2 a8, b8;
-      a8.x = f32x4_to_e4m3x4(x[j][0] * inv, x[j][1] * inv, x[j][2] * inv, x[j][3] * inv);
-      a8.y = f32x4_to_e4m3x4(x[j][4] * inv, x[j][5] * inv, x[j][6] * inv, x[j][7] * inv);
-      b8.x = f32x4_to_e4m3x4(x[j][8] * inv, x[j][9] * inv, x[j][10] * inv, x[j][11] * inv);
-      b8.y = f32x4_to_e4m3x4(x[j][12] * inv, x[j][13] * inv, x[j][14] * inv, x[j][15] * inv);
-      if (bad) a8 = b8 = make_uint2(0u, 0u);  // the scale says NaN; no code does
-      *reinterpret_cast<uint2*>(dst + o * D + i0) = a8;
-      *reinterpret_cast<uint2*>(dst + o * D + D / 2 + i0) = b8;
-    }
-  }
-  if (lane == 0) *sc = bad ? __int_as_float(0x7fffffff) : pow2i(e);
+  __syncthreads();  // red, and what was written here, may be used again
 }
 
 template <int D>
-__global__ void __launch_bounds__(kAppendThreads) rope_kv_append_fp8_kernel(const KvFp8Args a) {
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_kv_append_fp8_kernel(const KvFp8Args a) {
   // programmatic dependent launch: let the next kernel launch once every CTA
   // of this one runs, and wait for the previous kernel before touching memory
   grid_dep_launch();
   grid_dep_wait();
   constexpr int kLanes = D / 16;
-  constexpr int kWarps = kAppendThreads / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ uint32_t red[2][kAppendThreads / 32];
+  const int lane = threadIdx.x & 31;
   const int T = a.num_tokens;
 
   if ((int)blockIdx.x < a.kv_ctas) {
-    const int group = (int)blockIdx.x % a.head_groups;
-    const int t0 = (int)blockIdx.x / a.head_groups * a.window;
-    const int t1 = min(t0 + a.window, T);
-    for (int item = group * kWarps + warp; item < 2 * a.num_kv_heads;
-         item += a.head_groups * kWarps) {
-      const bool is_k = item < a.num_kv_heads;
-      const int h = is_k ? item : item - a.num_kv_heads;
-      int prev = t0 > 0 ? a.slots[t0 - 1] : -1;
-      prev = prev < 0 ? -1 : prev / kKvBlock;
-      for (int t = t0; t < t1;) {
-        // lanes 0-15 look at the next rows; `n` of them are in row t's block
-        const int slot = lane < kKvBlock && t + lane < T ? a.slots[t + lane] : -1;
-        const int blk_l = slot < 0 ? -1 : slot / kKvBlock;
-        const int blk = __shfl_sync(0xffffffffu, blk_l, 0);
-        const uint32_t in = __ballot_sync(0xffffffffu, lane < kKvBlock && blk_l == blk);
-        const int n = in == 0xffffu ? kKvBlock : __ffs(~in) - 1;
-        // a run belongs to the window that it starts in
-        if (blk < 0 || blk == prev) {
-          prev = blk;
-          t += blk < 0 ? 1 : n;
-          continue;
-        }
-        if (blk >= a.num_blocks) {
-          if (lane == 0) set_device_error(kDevBadIndex);
-          prev = blk;
-          t += n;
-          continue;
-        }
-        append_rows<D>(a, t, n, blk, slot, is_k, h);
-        t += n;
+    const int g0 = (int)blockIdx.x % a.group_ctas * a.groups_per_cta;
+    const int g1 = min(g0 + a.groups_per_cta, a.groups);
+    const int t0 = (int)blockIdx.x / a.group_ctas * kWindow;
+    const int t1 = min(t0 + kWindow, T);
+    int prev = t0 > 0 ? a.slots[t0 - 1] : -1;
+    prev = prev < 0 ? -1 : prev / kKvBlock;
+    // uniform over the CTA: every warp walks the same rows
+    for (int t = t0; t < t1;) {
+      // lanes 0-15 look at the next rows; n of them are in row t's block
+      const int slot = lane < kKvBlock && t + lane < T ? a.slots[t + lane] : -1;
+      const int blk_l = slot < 0 ? -1 : slot / kKvBlock;
+      const int blk = __shfl_sync(0xffffffffu, blk_l, 0);
+      const uint32_t in = __ballot_sync(0xffffffffu, lane < kKvBlock && blk_l == blk);
+      const int n = in == 0xffffu ? kKvBlock : __ffs(~in) - 1;
+      // a run belongs to the window that it starts in
+      if (blk < 0 || blk == prev || blk >= a.num_blocks || (n == 1 && a.single_ctas > 0)) {
+        if (blk >= a.num_blocks && threadIdx.x == 0) set_device_error(kDevBadIndex);
         prev = blk;
-        // more than 16 neighbouring rows of one block name some slot twice: go
-        // on in order, as a later call would
-        while (n == kKvBlock && t < T) {
-          __syncwarp();
-          const int s2 = lane < kKvBlock && t + lane < T ? a.slots[t + lane] : -1;
-          const int b2 = s2 < 0 ? -1 : s2 / kKvBlock;
-          const uint32_t in2 = __ballot_sync(0xffffffffu, lane < kKvBlock && b2 == blk);
-          const int n2 = in2 == 0xffffu ? kKvBlock : __ffs(~in2) - 1;
-          if (n2 == 0) break;
-          append_rows<D>(a, t, n2, blk, s2, is_k, h);
-          t += n2;
-          if (n2 < kKvBlock) break;
-        }
+        t += blk < 0 ? 1 : n;
+        continue;
+      }
+      append_rows<D>(a, t, n, blk, slot, g0, g1, red);
+      t += n;
+      prev = blk;
+      // more than 16 neighbouring rows of one block name some slot twice: go on in
+      // order, as a later call would
+      while (n == kKvBlock && t < T) {
+        const int s2 = lane < kKvBlock && t + lane < T ? a.slots[t + lane] : -1;
+        const int b2 = s2 < 0 ? -1 : s2 / kKvBlock;
+        const uint32_t in2 = __ballot_sync(0xffffffffu, lane < kKvBlock && b2 == blk);
+        const int n2 = in2 == 0xffffu ? kKvBlock : __ffs(~in2) - 1;
+        if (n2 == 0) break;
+        append_rows<D>(a, t, n2, blk, s2, g0, g1, red);
+        t += n2;
+        if (n2 < kKvBlock) break;
       }
     }
     return;
   }
 
-  // q rows: thread = 16 elements of a head
-  const int t = (int)blockIdx.x - a.kv_ctas;
-  int pos = a.positions[t];
-  const bool ok = pos >= 0 && pos < a.max_pos;
-  if (!ok) {
-    if (threadIdx.x == 0) set_device_error(kDevBadIndex);
-    pos = 0;
+  if ((int)blockIdx.x < a.kv_ctas + a.single_ctas) {
+    append_single<D>(a, (int64_t)((int)blockIdx.x - a.kv_ctas) * (kAppendThreads / kLanes) +
+                            threadIdx.x / kLanes);
+    return;
   }
+
+  // q rows: thread = 16 elements of a head; the next item's are loaded meanwhile
   const int items = a.num_q_heads * kLanes;
-  for (int base = 0; base < items; base += kAppendThreads) {  // uniform: the norm shuffles
-    const int item = base + threadIdx.x;
-    const bool live = item < items;
-    const int h = live ? item / kLanes : 0, i0 = (item % kLanes) * 8;
-    const __nv_bfloat16* row = a.qkv + (int64_t)t * a.qkv_stride + (int64_t)h * D;
-    const uint4 lo = *reinterpret_cast<const uint4*>(row + i0);
-    const uint4 hi = *reinterpret_cast<const uint4*>(row + D / 2 + i0);
+  const int tb = ((int)blockIdx.x - a.kv_ctas - a.single_ctas) * a.q_tokens;
+  const int total = min(a.q_tokens, T - tb) * items;
+  int t = 0, h = 0, pos = 0;
+  bool live = false;
+  uint4 lo, hi;
+  const int i0 = (threadIdx.x % kLanes) * 8;
+  auto load = [&](int i) {
+    live = i < total;
+    t = tb + (live ? i / items : 0);
+    h = live ? i % items / kLanes : 0;
+    const __nv_bfloat16* row = a.qkv + (int64_t)t * a.qkv_stride + (int64_t)h * D + i0;
+    lo = *reinterpret_cast<const uint4*>(row);
+    hi = *reinterpret_cast<const uint4*>(row + D / 2);
+    pos = a.positions[t];
+    if (pos < 0 || pos >= a.max_pos) {
+      if (live) set_device_error(kDevBadIndex);
+      live = false;
+      pos = 0;
+    }
+  };
+  load(threadIdx.x);
+  for (int base = 0; base < total; base += kAppendThreads) {  // uniform: the norm shuffles
     float x[16];
     unpack16(lo, hi, x);
-    if (a.q_norm_w != nullptr) head_norm<D>(x, a.q_norm_w, i0, a.qk_eps);
-    rotate16<D>(x, a.rope_cos, a.rope_sin, pos, i0);
-    if (live && ok) {
-      __nv_bfloat16* out = a.q_out + (int64_t)t * a.q_out_stride + (int64_t)h * D;
+    const Rope8 rp = load_rope<D>(a, pos, i0);
+    const bool store = live;
+    __nv_bfloat16* out = a.q_out + (int64_t)t * a.q_out_stride + (int64_t)h * D + i0;
+    if (base + kAppendThreads < total) load(base + kAppendThreads + threadIdx.x);
+    if (a.q_norm_w != nullptr) head_norm<D>(x, a.q_norm_w, i0, a.qk_eps, true);
+    rotate16(x, rp);
+    if (store) {
       uint4 l, g;
       l.x = pack_bf16x2(x[0], x[1]);
       l.y = pack_bf16x2(x[2], x[3]);
@@ -308,8 +415,8 @@ __global__ void __launch_bounds__(kAppendThreads) rope_kv_append_fp8_kernel(cons
       g.y = pack_bf16x2(x[10], x[11]);
       g.z = pack_bf16x2(x[12], x[13]);
       g.w = pack_bf16x2(x[14], x[15]);
-      *reinterpret_cast<uint4*>(out + i0) = l;
-      *reinterpret_cast<uint4*>(out + D / 2 + i0) = g;
+      *reinterpret_cast<uint4*>(out) = l;
+      *reinterpret_cast<uint4*>(out + D / 2) = g;
     }
   }
 }
@@ -368,15 +475,27 @@ extern "C" int muk_rope_kv_append_fp8(
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   a.num_blocks = num_blocks;
-  // One row per K/V CTA while the step is small (each row of a decode step is a
-  // run of its own); 16-row windows for large steps, whose rows are mostly one
-  // block's and would leave 15 of 16 single-row CTAs with nothing to do.
-  a.window = num_tokens > 1024 ? kKvBlock : 1;
-  a.head_groups = (2 * num_kv_heads + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-  const int64_t kv = (int64_t)((num_tokens + a.window - 1) / a.window) * a.head_groups;
-  MUK_REQUIRE(kv + num_tokens <= INT32_MAX, "muk_rope_kv_append_fp8: %d tokens", num_tokens);
+  const int heads = kAppendThreads * 16 / (kKvBlock * head_dim);
+  // Small steps are spread: a window's groups over as many CTAs, a q row a CTA, and rows
+  // that are alone in their block get lanes of their own (a window would do 16 of them
+  // one after the other: 29 us for 256 decode rows).  In large steps, whose rows mostly
+  // have neighbours, a CTA keeps a window or 8 q rows and loads ahead: with a CTA for
+  // each group and q row, 8k rows took 61 us.
+  const bool large = num_tokens > 1024;
+  a.groups = (2 * num_kv_heads + heads - 1) / heads;
+  a.groups_per_cta = large ? a.groups : 1;
+  a.group_ctas = (a.groups + a.groups_per_cta - 1) / a.groups_per_cta;
+  a.q_tokens = large ? 8 : 1;
+  const int64_t kv = (int64_t)((num_tokens + kWindow - 1) / kWindow) * a.group_ctas;
+  const int64_t single = large ? 0
+                               : ((int64_t)num_tokens * 2 * num_kv_heads * (head_dim / 16) +
+                                  kAppendThreads - 1) / kAppendThreads;
+  const int64_t q_ctas = (num_tokens + a.q_tokens - 1) / a.q_tokens;
+  MUK_REQUIRE(kv + single + q_ctas <= INT32_MAX && (int64_t)num_q_heads * head_dim <= (1 << 24),
+              "muk_rope_kv_append_fp8: %d tokens of %d heads", num_tokens, num_q_heads);
   a.kv_ctas = (int)kv;
-  const dim3 grid((unsigned)(kv + num_tokens));
+  a.single_ctas = (int)single;
+  const dim3 grid((unsigned)(kv + single + q_ctas));
   launch_pdl(head_dim == 128 ? rope_kv_append_fp8_kernel<128> : rope_kv_append_fp8_kernel<64>, grid,
              dim3(kAppendThreads), 0, as_stream(stream), a);
   return check_launch("muk_rope_kv_append_fp8");
