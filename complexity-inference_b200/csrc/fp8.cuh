@@ -5,7 +5,8 @@
 // inside f16), so the attention kernels multiply f16 x f16 into f32: K and V
 // enter without rounding, the softmax weights keep 11 bits instead of bf16's 8,
 // and q (bf16) is scaled by a power of two per head row so that it fits f16
-// exactly except for elements more than 2^29 below the row's largest.
+// exactly except for elements more than 2^29 below the row's largest.  (Decode's
+// scores multiply the codes themselves, see attention_fp8.cu.)
 #pragma once
 
 #include <cuda_fp16.h>
@@ -75,12 +76,12 @@ __device__ __forceinline__ float2 unpack_f16x2(uint32_t v) {
 }
 
 // The factor 2^f that brings a row whose largest |x| has these bits into
-// [2^14, 2^15) (f held to what an f32 can scale by; zero and non-finite rows: 1),
+// [2^to, 2^(to + 1)) (f held to what an f32 can scale by; zero and non-finite rows: 1),
 // and its inverse.
-__device__ __forceinline__ void row_factor(uint32_t max_bits, float& up, float& down) {
+__device__ __forceinline__ void row_factor(uint32_t max_bits, int to, float& up, float& down) {
   const int x = (int)(max_bits >> 23);           // biased exponent
-  int f = (x == 0 || x == 255) ? 0 : 14 - (x - 127);
-  f = f > 126 ? 126 : (f < -113 ? -113 : f);
+  int f = (x == 0 || x == 255) ? 0 : to - (x - 127);
+  f = f > 126 ? 126 : (f < -126 ? -126 : f);
   up = pow2i(f);
   down = pow2i(-f);
 }

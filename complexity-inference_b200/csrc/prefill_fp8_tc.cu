@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
           top = max(top, max((w[u] << 16) & 0x7fffffffu, w[u] & 0x7fff0000u));
       }
       float up, down;
-      row_factor(top, up, down);
+      row_factor(top, 14, up, down);
       c = down * a.scale_log2;
       uint8_t* qrow = basep + XLayout::kQ + qi * 2 * kXQPanel + r * 128;
 #pragma unroll
