@@ -10,10 +10,10 @@
 // :184-245 (pre-norm, GQA attention with RoPE, SwiGLU MLP, mu_clamp at the
 // embedding, every norm output, the attention and MLP outputs and the layer
 // output) over the flat step batch.
-#include <math.h>
 #include <stdint.h>
 
 #include "abi_util.h"
+#include "kv_step.h"
 
 using namespace muk;
 
@@ -35,45 +35,26 @@ extern "C" int muk_llama_forward(const MukLlamaModel* m, const MukStepBatch* b, 
   MUK_REQUIRE(m->lm_rows > 0 && m->lm_rows <= m->vocab && m->logits_ld >= m->lm_rows,
               "muk_llama_forward: LM head rows %d / logits stride %lld (vocab %d)", m->lm_rows,
               (long long)m->logits_ld, m->vocab);
-  const int T = b->num_tokens, B = b->num_seqs, nd = b->num_decode;
+  MUK_REQUIRE(!m->kv_scales || !m->fused_rope,
+              "muk_llama_forward: an 8-bit KV cache needs fused_rope = 0");
+  const int T = b->num_tokens, B = b->num_seqs;
   const int H = m->hidden, Hq = m->num_q_heads, Hkv = m->num_kv_heads, D = m->head_dim;
   const int qkv_n = (Hq + 2 * Hkv) * D, attn_n = Hq * D;
   const int cl = m->clamp;
   const float mu = m->mu, cmin = m->clamp_min, cmax = m->clamp_max;
-  const float scale = 1.0f / sqrtf((float)D);
   // bf16 buffers, addressed in 2-byte elements
   auto* qkv = static_cast<uint16_t*>(m->qkv);
   auto* attn = static_cast<uint16_t*>(m->attn);
   auto* x = static_cast<uint16_t*>(m->x);
-  const int64_t layer_elems = (int64_t)m->num_blocks * Hkv * m->block_size * D;
-  auto* pool = static_cast<uint16_t*>(m->kv_pool);
 
   MUK_TRY(muk_embed(b->input_ids, m->embed, H, m->resid, T, H, m->vocab, cl, mu, cmin, cmax,
                     stream));
   MUK_TRY(muk_residual_rmsnorm(m->resid, nullptr, 0, 0, 0, nullptr, m->layers[0].in_norm, m->eps,
                                x, m->x_stride, T, H, 0, 0, cl, mu, cmin, cmax, stream));
 
-  // Paged decode attention over the decode rows, varlen prefill attention
-  // over the rest (decode sequences own one row each, so prefill starts at nd).
-  auto attention = [&](int l, void* kc, void* vc) -> int {
-    (void)l;
-    if (nd > 0) {
-      int bound = b->decode_len_bound;
-      const int bt_cap = b->block_table_stride * m->block_size;
-      if (bound > bt_cap) bound = bt_cap;
-      MUK_TRY(muk_paged_decode_attn(qkv, qkv_n, attn, attn_n, kc, vc, b->block_tables,
-                                    b->block_table_stride, b->seq_lens, nd, Hq, Hkv, D,
-                                    m->block_size, m->num_blocks, scale, bound, m->attn_ws,
-                                    m->attn_ws_bytes, stream));
-    }
-    if (B > nd) {
-      MUK_TRY(muk_paged_prefill_attn(qkv + (int64_t)nd * qkv_n, qkv_n, attn + (int64_t)nd * attn_n,
-                                     attn_n, kc, vc, b->block_tables + (int64_t)nd * b->block_table_stride,
-                                     b->block_table_stride, b->seq_lens + nd, b->prefill_cu,
-                                     B - nd, b->max_q_len, Hq, Hkv, D, m->block_size,
-                                     m->num_blocks, scale, stream));
-    }
-    return MUK_OK;
+  // The KV append and attention of layer l are kv_append / kv_attention (kv_step.h).
+  auto attention = [&](const KvLayer& kv) -> int {
+    return kv_attention(m, b, kv, nullptr, stream);
   };
 
   // Sum a row-parallel projection over the tensor-parallel ranks; returns the
@@ -96,14 +77,13 @@ extern "C" int muk_llama_forward(const MukLlamaModel* m, const MukStepBatch* b, 
     const MukRowNorm rn = {m->sumsq, (int64_t)T, H / 128, H, m->eps};
     for (int l = 0; l < m->num_layers; ++l) {
       const MukLlamaLayer& L = m->layers[l];
-      void* kc = pool + (int64_t)(2 * l) * layer_elems;
-      void* vc = pool + (int64_t)(2 * l + 1) * layer_elems;
+      const KvLayer kv = kv_layer(m, l);
       MUK_TRY(muk_gemm_qkv_rope_rownorm(x, m->x_stride, L.wqkv, H, qkv, qkv_n, T, H, b->positions,
                                         b->slot_mapping, m->rope_cos, m->rope_sin, m->rope_len,
-                                        Hq, Hkv, D, nullptr, nullptr, 1e-6f, kc, vc,
+                                        Hq, Hkv, D, nullptr, nullptr, 1e-6f, kv.k, kv.v,
                                         m->num_blocks, m->block_size, l > 0 ? &rn : nullptr,
                                         stream));
-      MUK_TRY(attention(l, kc, vc));
+      MUK_TRY(attention(kv));
       MUK_TRY(muk_gemm_residual_norm(attn, attn_n, L.wo, attn_n, T, H, attn_n, m->resid, H,
                                      L.post_norm, x, m->x_stride, m->sumsq, T, stream));
       MUK_TRY(muk_gemm_swiglu_rownorm(x, m->x_stride, L.wgu, H, m->act, m->inter_pad, T,
@@ -122,17 +102,15 @@ extern "C" int muk_llama_forward(const MukLlamaModel* m, const MukStepBatch* b, 
   }
 
   // q|k|v projection with RoPE and the KV append (fused or as two kernels)
-  auto qkv_proj = [&](const MukLlamaLayer& L, void* kc, void* vc) -> int {
+  auto qkv_proj = [&](const MukLlamaLayer& L, const KvLayer& kv) -> int {
     if (m->fused_rope)
       return muk_gemm_qkv_rope(x, m->x_stride, L.wqkv, H, qkv, qkv_n, T, H, b->positions,
                                b->slot_mapping, m->rope_cos, m->rope_sin, m->rope_len, Hq, Hkv, D,
-                               nullptr, nullptr, 1e-6f, kc, vc, m->num_blocks, m->block_size,
+                               nullptr, nullptr, 1e-6f, kv.k, kv.v, m->num_blocks, m->block_size,
                                stream);
     MUK_TRY(muk_gemm_bf16(x, m->x_stride, L.wqkv, H, qkv, qkv_n, T, qkv_n, H, kEpiBf16, 1, nullptr,
                           stream));
-    return muk_rope_kv_append(qkv, qkv_n, b->positions, b->slot_mapping, m->rope_cos, m->rope_sin,
-                              m->rope_len, T, Hq, Hkv, D, nullptr, nullptr, 1e-6f, kc, vc,
-                              m->num_blocks, m->block_size, stream);
+    return kv_append(m, b, kv, nullptr, nullptr, stream);
   };
 
   if (m->tp_world > 1 && m->tp_norm) {
@@ -156,10 +134,9 @@ extern "C" int muk_llama_forward(const MukLlamaModel* m, const MukStepBatch* b, 
     };
     for (int l = 0; l < m->num_layers; ++l) {
       const MukLlamaLayer& L = m->layers[l];
-      void* kc = pool + (int64_t)(2 * l) * layer_elems;
-      void* vc = pool + (int64_t)(2 * l + 1) * layer_elems;
-      MUK_TRY(qkv_proj(L, kc, vc));
-      MUK_TRY(attention(l, kc, vc));
+      const KvLayer kv = kv_layer(m, l);
+      MUK_TRY(qkv_proj(L, kv));
+      MUK_TRY(attention(kv));
       MUK_TRY(project_norm(attn, attn_n, L.wo, attn_n, L.post_norm, 0));
       MUK_TRY(muk_gemm_bf16(x, m->x_stride, L.wgu, H, m->act, m->inter_pad, T, 2 * m->inter_pad,
                             H, kEpiSwiglu, 1, nullptr, stream));
@@ -174,21 +151,9 @@ extern "C" int muk_llama_forward(const MukLlamaModel* m, const MukStepBatch* b, 
 
   for (int l = 0; l < m->num_layers; ++l) {
     const MukLlamaLayer& L = m->layers[l];
-    void* kc = pool + (int64_t)(2 * l) * layer_elems;
-    void* vc = pool + (int64_t)(2 * l + 1) * layer_elems;
-    if (m->fused_rope) {
-      MUK_TRY(muk_gemm_qkv_rope(x, m->x_stride, L.wqkv, H, qkv, qkv_n, T, H, b->positions,
-                                b->slot_mapping, m->rope_cos, m->rope_sin, m->rope_len, Hq, Hkv,
-                                D, nullptr, nullptr, 1e-6f, kc, vc, m->num_blocks, m->block_size,
-                                stream));
-    } else {
-      MUK_TRY(muk_gemm_bf16(x, m->x_stride, L.wqkv, H, qkv, qkv_n, T, qkv_n, H, kEpiBf16, 1,
-                            nullptr, stream));
-      MUK_TRY(muk_rope_kv_append(qkv, qkv_n, b->positions, b->slot_mapping, m->rope_cos,
-                                 m->rope_sin, m->rope_len, T, Hq, Hkv, D, nullptr, nullptr, 1e-6f,
-                                 kc, vc, m->num_blocks, m->block_size, stream));
-    }
-    MUK_TRY(attention(l, kc, vc));
+    const KvLayer kv = kv_layer(m, l);
+    MUK_TRY(qkv_proj(L, kv));
+    MUK_TRY(attention(kv));
     // O projection (split-K f32 partials) -> reduce -> h += clamp(o); x = clamp(norm(h))
     int np;
     if (fused_tp) {

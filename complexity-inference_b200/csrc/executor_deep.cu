@@ -13,10 +13,10 @@
 // velocity / state update, mu_clamp), the token-routed MLP (layers.py:427-559:
 // expert = mu-guided route of the token, SwiGLU experts) and the clamped
 // residual stream.
-#include <math.h>
 #include <stdint.h>
 
 #include "abi_util.h"
+#include "kv_step.h"
 
 using namespace muk;
 
@@ -59,6 +59,8 @@ extern "C" int muk_deep_forward(const MukDeepModel* m, const MukStepBatch* b, in
   MUK_REQUIRE(m->lm_rows > 0 && m->lm_rows <= m->vocab && m->logits_ld >= m->lm_rows,
               "muk_deep_forward: LM head rows %d / logits stride %lld (vocab %d)", m->lm_rows,
               (long long)m->logits_ld, m->vocab);
+  MUK_REQUIRE(!m->kv_scales || !m->fused_rope,
+              "muk_deep_forward: an 8-bit KV cache needs fused_rope = 0");
   MUK_REQUIRE(m->x_stride >= 2 * (int64_t)m->hidden, "muk_deep_forward: x stride %lld < 2 x %d",
               (long long)m->x_stride, m->hidden);
   MUK_REQUIRE(m->ctrl_hidden > 0, "muk_deep_forward: controller width %d", m->ctrl_hidden);
@@ -68,21 +70,18 @@ extern "C" int muk_deep_forward(const MukDeepModel* m, const MukStepBatch* b, in
               "muk_deep_forward: experts [%d, %d) of %d on %d rank(s)", e0, e0 + El, E,
               m->tp_world);
 
-  const int T = b->num_tokens, B = b->num_seqs, nd = b->num_decode;
+  const int T = b->num_tokens, B = b->num_seqs;
   const int H = m->hidden, Hq = m->num_q_heads, Hkv = m->num_kv_heads, D = m->head_dim;
   const int C = m->ctrl_hidden, I = m->inter_pad;
   const int qkv_n = (Hq + 2 * Hkv) * D, attn_n = Hq * D;
   const int cl = m->clamp;
   const float mu = m->mu, cmin = m->clamp_min, cmax = m->clamp_max, eps = m->eps;
-  const float scale = 1.0f / sqrtf((float)D);
   const int64_t ldx = m->x_stride, TH = (int64_t)T * H;
   // bf16 buffers, addressed in 2-byte elements
   auto* x = static_cast<uint16_t*>(m->x);
   auto* hv = static_cast<uint16_t*>(m->hv);
   auto* qkv = static_cast<uint16_t*>(m->qkv);
   auto* attn = static_cast<uint16_t*>(m->attn);
-  const int64_t layer_elems = (int64_t)m->num_blocks * Hkv * m->block_size * D;
-  auto* pool = static_cast<uint16_t*>(m->kv_pool);
   const int rank = m->tp_rank, world = m->tp_world;
   // GEMM + all-reduce in one kernel for steps of up to tp_fused rows
   const bool fused_tp = world > 1 && m->tp_fused > 0 && T <= m->tp_fused;
@@ -115,8 +114,7 @@ extern "C" int muk_deep_forward(const MukDeepModel* m, const MukStepBatch* b, in
 
   for (int l = 0; l < m->num_layers; ++l) {
     const MukDeepLayer& L = m->layers[l];
-    void* kc = pool + (int64_t)(2 * l) * layer_elems;
-    void* vc = pool + (int64_t)(2 * l + 1) * layer_elems;
+    const KvLayer kv = kv_layer(m, l);
     // layer 0 has no mu_prev: its projection and controller read the first
     // H columns of [x | mu_prev] and [h | v] (deep.py:296, layers.py:99-100)
     const int kdim = l == 0 ? H : 2 * H;
@@ -125,35 +123,15 @@ extern "C" int muk_deep_forward(const MukDeepModel* m, const MukStepBatch* b, in
     if (m->fused_rope) {
       MUK_LAUNCH(1, muk_gemm_qkv_rope(x, ldx, L.wcat, 2 * H, qkv, qkv_n, T, kdim, b->positions,
                                       b->slot_mapping, m->rope_cos, m->rope_sin, m->rope_len, Hq,
-                                      Hkv, D, L.q_norm, L.k_norm, 1e-6f, kc, vc, m->num_blocks,
+                                      Hkv, D, L.q_norm, L.k_norm, 1e-6f, kv.k, kv.v, m->num_blocks,
                                       m->block_size, stream));
     } else {
       MUK_LAUNCH(1, muk_gemm_bf16(x, ldx, L.wcat, 2 * H, qkv, qkv_n, T, qkv_n, kdim, MUK_EPI_BF16,
                                   1, nullptr, stream));
-      MUK_LAUNCH(1, muk_rope_kv_append(qkv, qkv_n, b->positions, b->slot_mapping, m->rope_cos,
-                                       m->rope_sin, m->rope_len, T, Hq, Hkv, D, L.q_norm,
-                                       L.k_norm, 1e-6f, kc, vc, m->num_blocks, m->block_size,
-                                       stream));
+      MUK_LAUNCH(1, kv_append(m, b, kv, L.q_norm, L.k_norm, stream));
     }
 
-    // paged decode attention over the decode rows, varlen prefill over the
-    // rest (decode sequences own one row each, so prefill rows start at nd)
-    if (nd > 0) {
-      int bound = b->decode_len_bound;
-      const int bt_cap = b->block_table_stride * m->block_size;
-      if (bound > bt_cap) bound = bt_cap;
-      MUK_LAUNCH(2, muk_paged_decode_attn(qkv, qkv_n, attn, attn_n, kc, vc, b->block_tables,
-                                          b->block_table_stride, b->seq_lens, nd, Hq, Hkv, D,
-                                          m->block_size, m->num_blocks, scale, bound, m->attn_ws,
-                                          m->attn_ws_bytes, stream));
-    }
-    if (B > nd) {
-      MUK_LAUNCH(1, muk_paged_prefill_attn(
-                        qkv + (int64_t)nd * qkv_n, qkv_n, attn + (int64_t)nd * attn_n, attn_n, kc,
-                        vc, b->block_tables + (int64_t)nd * b->block_table_stride,
-                        b->block_table_stride, b->seq_lens + nd, b->prefill_cu, B - nd,
-                        b->max_q_len, Hq, Hkv, D, m->block_size, m->num_blocks, scale, stream));
-    }
+    MUK_TRY(kv_attention(m, b, kv, &cnt.n, stream));
 
     // h = mu_clamp(o_proj(attn)) in f32 (INL input) and bf16 (hv[:, :H],
     // the controller / mu projection input)

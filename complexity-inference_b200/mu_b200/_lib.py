@@ -154,7 +154,7 @@ class MukLlamaModel(ctypes.Structure):
                 ("ar_scratch", c_void_p * 8), ("ar_flags", c_void_p * 8), ("fused_rope", c_int),
                 ("tp_fused", c_int), ("fused_norm", c_int), ("sumsq", c_void_p),
                 ("tp_norm", c_int), ("x_peer", c_void_p * 8), ("lm_rows", c_int),
-                ("logits_ld", c_int64), ("tp_push_bf16", c_int)]
+                ("logits_ld", c_int64), ("tp_push_bf16", c_int), ("kv_scales", c_void_p)]
 
 
 class MukDeepLayer(ctypes.Structure):
@@ -183,7 +183,7 @@ class MukDeepModel(ctypes.Structure):
                 ("lm_rows", c_int), ("attn_ws", c_void_p), ("attn_ws_bytes", c_size_t),
                 ("fused_rope", c_int), ("tp_world", c_int), ("tp_rank", c_int),
                 ("tp_fused", c_int), ("ar_data", c_void_p * 8), ("ar_scratch", c_void_p * 8),
-                ("ar_flags", c_void_p * 8)]
+                ("ar_flags", c_void_p * 8), ("kv_scales", c_void_p)]
 
 
 class MukStepBatch(ctypes.Structure):

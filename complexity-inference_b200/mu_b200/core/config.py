@@ -158,13 +158,16 @@ class ModelConfig:
 
 @dataclass
 class CacheConfig:
-    """Paged KV cache settings (config.py:221-245)."""
+    """Paged KV cache settings (config.py:221-245).
+
+    ``dtype`` "float8_e4m3" (not in the reference) makes the paged pool 8-bit, with a
+    scale for each (block, head); any other value keeps it bf16."""
 
     max_seq_len: int = 2048
     block_size: int = 16
     max_num_blocks: int = 2048
     max_num_seqs: int = 256
-    dtype: Literal["float16", "bfloat16", "float32"] = "float16"
+    dtype: Literal["float16", "bfloat16", "float32", "float8_e4m3"] = "float16"
     use_paged: bool = True
     mu_enabled: bool = True
     num_gpu_blocks: Optional[int] = None

@@ -122,7 +122,17 @@ class Workspace:
                                                             dtype=f32)
         nbytes = K.decode_attn_workspace_size(max_seqs, Hq, D, max_seq_len)
         self.attn_ws = torch.empty(max(nbytes // 4, 4), device=dev, dtype=f32)
+        self.attn_ws_fp8: Optional[torch.Tensor] = None
+        if model.kv_quantized:
+            self.add_fp8(cfg, dev)
         model.extra_workspace(self, T)
+
+    def add_fp8(self, cfg, dev) -> None:
+        """The decode attention's scratch for an 8-bit cache."""
+        if self.attn_ws_fp8 is None:
+            nbytes = K.decode_attn_fp8_workspace_size(self.max_seqs, cfg.num_attention_heads,
+                                                      cfg.head_dim, self.max_seq_len)
+            self.attn_ws_fp8 = torch.empty(max(nbytes // 4, 4), device=dev, dtype=torch.float32)
 
     def part_view(self, splits: int, rows: int, cols: int) -> torch.Tensor:
         return self.part[: splits * rows * cols].view(splits, rows, cols)
@@ -146,6 +156,7 @@ class MuModelBase:
         self._rope_len = 0
         self._fused_rope = os.environ.get("MU_FUSED_ROPE", "1") != "0"
         self._tp_fused = os.environ.get("MU_TP_FUSED", "1") != "0"
+        self.kv_quantized = False  # 8-bit KV cache (set with the cache, see use_cache)
         self.tp_group = None   # torch.distributed group when tensor-parallel
         self.comm = None       # mu_b200.comm.PeerAllReduce when tensor-parallel over NVLink
         self.ensure_rope(max(config.max_position_embeddings, 16))
@@ -218,6 +229,17 @@ class MuModelBase:
         self.ensure_rope(max_seq_len + 1)
         return True
 
+    def use_cache(self, cache) -> None:
+        """Follow the cache's kind: an 8-bit one takes its own append and attention
+        kernels, and the decode attention scratch of another size (added to the
+        workspace, whose other buffers stay: captured graphs hold their addresses)."""
+        if cache.quantized and (cache.head_dim not in (64, 128) or cache.block_size != 16):
+            raise ValueError(f"float8_e4m3 KV cache: head_dim {cache.head_dim} / block_size "
+                             f"{cache.block_size} not built (64 or 128 / 16)")
+        self.kv_quantized = cache.quantized
+        if cache.quantized and self.ws is not None:
+            self.ws.add_fp8(self.config, self.device)
+
     # ---- shared pieces of the step ---------------------------------------------
     def row_parallel(self, A: torch.Tensor, W: torch.Tensor, T: int, N: int) -> torch.Tensor:
         """A row-parallel projection (O, down) summed over the TP ranks; returns
@@ -252,8 +274,9 @@ class MuModelBase:
         return part
 
     def fused_rope(self) -> bool:
-        """RoPE + KV append in the q|k|v GEMM's epilogue (MU_FUSED_ROPE=0: separate kernel)."""
-        return self._fused_rope and self.config.head_dim in (64, 128)
+        """RoPE + KV append in the q|k|v GEMM's epilogue (MU_FUSED_ROPE=0: separate kernel;
+        an 8-bit cache always takes one: a block's scale needs all of its rows)."""
+        return self._fused_rope and self.config.head_dim in (64, 128) and not self.kv_quantized
 
     def qkv_proj(self, layer: int, x: torch.Tensor, w: torch.Tensor, batch, cache,
                  q_norm_w=None, k_norm_w=None, rownorm=None) -> None:
@@ -270,6 +293,11 @@ class MuModelBase:
             return
         assert rownorm is None, "row-norm scaling needs the fused q|k|v epilogue"
         K.gemm(x, w, ws.qkv, K.MUK_EPI_BF16, M=T)
+        if cache.quantized:
+            K.rope_kv_append_fp8(ws.qkv, batch.positions, batch.slot_mapping, self.rope_cos,
+                                 self.rope_sin, Hq, Hkv, D, kc, vc, cache.k_scale(layer),
+                                 cache.v_scale(layer), q_norm_w, k_norm_w, 1e-6, num_tokens=T)
+            return
         K.rope_kv_append(ws.qkv, batch.positions, batch.slot_mapping, self.rope_cos, self.rope_sin,
                          Hq, Hkv, D, kc, vc, q_norm_w, k_norm_w, 1e-6, num_tokens=T)
 
@@ -281,6 +309,18 @@ class MuModelBase:
         kc, vc = cache.k_cache(layer), cache.v_cache(layer)
         nd, B = batch.num_decode, batch.num_seqs
         bt = batch.block_tables
+        if cache.quantized:
+            ks, vs = cache.k_scale(layer), cache.v_scale(layer)
+            if nd > 0:
+                bound = min(batch.decode_len_bound, bt.shape[1] * 16)
+                K.decode_attn_fp8(ws.qkv[:, : Hq * D], ws.attn, kc, vc, ks, vs, bt, batch.seq_lens,
+                                  Hq, Hkv, D, bound, workspace=ws.attn_ws_fp8, num_seqs=nd)
+            if B > nd:
+                T = batch.num_tokens
+                K.prefill_attn_fp8(ws.qkv[nd:T, : Hq * D], ws.attn[nd:T], kc, vc, ks, vs, bt[nd:],
+                                   batch.seq_lens[nd:], batch.prefill_cu, batch.max_q_len, Hq, Hkv,
+                                   D, num_seqs=B - nd)
+            return ws.attn
         if nd > 0:
             bound = min(batch.decode_len_bound, bt.shape[1] * 16)
             K.decode_attn(ws.qkv[:, : Hq * D], ws.attn, kc, vc, bt, batch.seq_lens, Hq, Hkv, D,

@@ -251,7 +251,7 @@ class StepEngine:
         worst = len(out.decode_requests) + sum(n // bs + 2 for _, n in out.prefill_chunks)
         if worst > free:
             for req in self.scheduler.fit_blocks(out, free, need_of,
-                                                 lambda r: len(cache.block_table(r.request_id))):
+                                                 lambda r: cache.held_blocks(r.request_id)):
                 self._release(req.request_id)
         prefills: List[Request] = []
         chunks: List[tuple] = []

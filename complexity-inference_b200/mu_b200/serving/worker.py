@@ -199,9 +199,10 @@ class MuWorker:
     def _init_cache(self) -> None:
         mc, cc, sc = self.model.config, self.config.cache, self.config.scheduler
         nblocks = cc.num_gpu_blocks or cc.max_num_blocks
+        dtype = torch.float8_e4m3fn if cc.dtype == "float8_e4m3" else torch.bfloat16
         self.cache = PagedKVCache(mc.num_hidden_layers, mc.num_key_value_heads, mc.head_dim,
-                                  cc.block_size, nblocks, torch.bfloat16, str(self.device),
-                                  self.config.mu)
+                                  cc.block_size, nblocks, dtype, str(self.device), self.config.mu)
+        self.model.use_cache(self.cache)
         max_len = self.config.max_seq_len_hint or cc.max_seq_len
         max_blocks = (max_len + cc.block_size - 1) // cc.block_size + 1
         max_seqs = max(cc.max_num_seqs, sc.max_batch_size)
@@ -228,6 +229,15 @@ class MuWorker:
         if not self.cache.allocate(request_id):
             return False
         self.active_requests[request_id] = {"seq_len": 0}
+        return True
+
+    def fork_request(self, parent_id: str, child_id: str) -> bool:
+        """A new request that continues from ``parent_id``'s cached tokens (its blocks
+        shared, the last one copied); False when the pool has no block for it."""
+        st = self.active_requests.get(parent_id)
+        if st is None or not self.cache.fork(parent_id, child_id):
+            return False
+        self.active_requests[child_id] = dict(st)
         return True
 
     def free_request(self, request_id: str) -> None:

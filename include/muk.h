@@ -680,6 +680,8 @@ typedef struct {
   int lm_rows;      /* rows of lm_head computed here (vocab, or this rank's vocabulary slice) */
   int64_t logits_ld; /* row stride of logits (vocab unless the slice sits in a wider buffer) */
   int tp_push_bf16; /* tp_norm: the projection rows travel to their owners as bf16 */
+  float* kv_scales; /* [layers][2][num_blocks][num_kv_heads]: kv_pool is an 8-bit cache (e4m3
+                       codes; fused_rope and fused_norm off); NULL: bf16 */
 } MukLlamaModel;
 
 /* The packed step (StepPacker layout; device pointers). */
@@ -790,6 +792,7 @@ typedef struct {
   float* ar_data[8];
   float* ar_scratch[8];
   uint32_t* ar_flags[8];
+  float* kv_scales; /* as in MukLlamaModel */
 } MukDeepModel;
 
 /* The whole forward step of a DeepForCausalLM (embedding; per layer the
