@@ -54,8 +54,10 @@ constexpr int kXStages = 3;          // converted steps: V(t) and K(t + 2)
 constexpr int kXRing = 3;            // steps (a V and a K tile) of codes on their way
 constexpr int kXFmaMask = 2;         // of 16 weights those i + 1 with (i & mask) == mask, i even: a quarter
 constexpr int kXItem = kXKeys * 128; // bytes of such a tile
-// Tiles of block constants: the loader is at most kXRing + kXStages + 1 tiles ahead of a
-// softmax warp.
+// Tiles of block constants: step t of the loader leaves those of tile t + 2 once the
+// conversion has freed the ring slot of step t - kXRing, so both issuers the stage of step
+// t - kXRing - kXStages, whose weights every softmax warp had then written: no warp reads
+// constants older than those of tile t - kXRing - kXStages + 1.
 constexpr int kXConsts = 16;
 static_assert(kXConsts > kXRing + kXStages + 2, "block constants are overwritten in use");
 constexpr int kXQPanel = 128 * 128;  // [128 rows][64 f16], one swizzled panel of a query tile
@@ -339,9 +341,10 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     // ---- loads of codes -------------------------------------------------------
     // Step t brings V(t) and K(t + 2), which the multiplies of one step need (steps -2
     // and -1: K alone): lanes 0-3 a block of V each, 4-7 one of K, 2 KB a copy.  Blocks
-    // behind the last key are left out (their rows become zero when converted).  Lanes 0-3
-    // also leave the constants of their block of tile t (ks, log2 vs, 1 / vs) for the
-    // softmax warps, whose S(t) comes after the conversion of these codes.
+    // behind the last key are left out (their rows become zero when converted).  Lanes 4-7
+    // also leave the constants of their block of tile t + 2 (ks, log2 vs, 1 / vs) for the
+    // softmax warps, before this warp's arrival on the codes: S(t + 2) comes after the
+    // conversion of the K codes of this step.
     const bool mine_k = lane >= 4;
     const uint8_t* src = (mine_k ? a.k_cache : a.v_cache) + (int64_t)kvh * (kKvBlock * kXD);
     const int64_t blk_bytes = (int64_t)a.num_kv_heads * (kKvBlock * kXD);
@@ -354,14 +357,14 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       const int blk = block_of(t);
       return blk >= 0 ? __ldg(bt + blk) : 0;
     };
-    auto scales_of = [&](int t, int i) {             // of this lane's block of tile t (lanes 0-3)
+    auto scales_of = [&](int t, int i) {             // of this lane's block of tile t + 2 (lanes 4-7)
       const int64_t at = (int64_t)(i >= 0 && i < a.num_blocks ? i : 0) * a.num_kv_heads + kvh;
-      return lane < 4 && block_of(t) >= 0 ? make_float2(__ldg(a.k_scale + at), __ldg(a.v_scale + at))
+      return mine_k && block_of(t) >= 0 ? make_float2(__ldg(a.k_scale + at), __ldg(a.v_scale + at))
                                           : make_float2(1.f, 1.f);
     };
     float4* consts = reinterpret_cast<float4*>(basep + XLayout::kScale);
     int id = id_of(-2), id_next = id_of(-1), slot = 0, issued = 0;
-    float2 scales = make_float2(1.f, 1.f);           // of tile t
+    float2 scales = scales_of(-2, id);
     uint32_t ph = 1;
     for (int t = -2; t < nt; ++t) {
       if (!x_wait(raw_empty + slot, ph, kDevTimeoutEmpty)) break;
@@ -371,22 +374,23 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
         set_device_error(kDevBadIndex);
         id = 0;
       }
-      if (t >= 0 && lane < 4) {
-        const float ks = clamp_scale(scales.x), vs = clamp_scale(scales.y);
-        float lv, iv;
-        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(vs));  // exact for powers of two
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(iv) : "f"(vs));
-        consts[(t % kXConsts) * 4 + lane] = make_float4(ks, lv, iv, 0.f);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(raw_full + slot, (uint32_t)(blocks * 2048));
-      __syncwarp();
+      // The copies go first (their bytes may arrive before they are expected: the phase
+      // still lacks this warp's arrival), so that they overlap the loads of the scales.
       if (have)
         asm volatile(
             "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 2048, [%2];\n" ::"r"(
                 dst + (uint32_t)(slot * 2 * kXItem)),
             "l"(src + id * blk_bytes), "r"(smem_u32(raw_full + slot))
             : "memory");
+      if (mine_k && lane < 8 && t + 2 < nt) {
+        const float ks = clamp_scale(scales.x), vs = clamp_scale(scales.y);
+        float lv, iv;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(vs));  // exact for powers of two
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(iv) : "f"(vs));
+        consts[((t + 2) % kXConsts) * 4 + (lane & 3)] = make_float4(ks, lv, iv, 0.f);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(raw_full + slot, (uint32_t)(blocks * 2048));
       ++issued;
       id = id_next;
       id_next = id_of(t + 2);

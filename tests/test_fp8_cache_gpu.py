@@ -260,6 +260,37 @@ def test_prefill_long(cuda, past, n, gain):
         _near(outs[0][lo:hi], want, bound, f"rows {lo}..{hi}")
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (16, 2, 128), (8, 4, 64)])
+def test_prefill_cold(cuda, hq, hkv, d):
+    """Every row of prompts whose codes and scales come from memory (the L2 cache holds
+    other data), each block under a scale of its own; the launch before it saw other
+    scales and codes, so nothing that it left in shared memory can pass for these."""
+    cases = [(0, 900), (300, 500), (0, 64), (1500, 130), (0, 1), (77, 700)]
+    lens, qn = [p + n for p, n in cases], [n for _, n in cases]
+    cu = [0]
+    for n in qn:
+        cu.append(cu[-1] + n)
+    junk = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    for turn in range(4):
+        bt, nb = _tables(lens, 100 + turn)
+        kc, ks = _quantised(nb, hkv, d, 40 + turn, spread=1.0 + turn)
+        vc, vs = _quantised(nb, hkv, d, 50 + turn, spread=4.0 - turn)
+        q = (0.2 * torch.randn(cu[-1], hq * d, device="cuda", generator=_gen(60 + turn))).bfloat16()
+        sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        out = torch.empty_like(q)
+        junk.fill_(turn)
+        _k().prefill_attn_fp8(q, out, kc, vc, ks, vs, bt, sl, cud, max(qn), hq, hkv, d)
+        assert _err() == 0
+        for b, (past, n) in enumerate(cases):
+            for lo in range(0, n, 128):
+                hi = min(lo + 128, n)
+                rows = slice(cu[b] + lo, cu[b] + hi)
+                want, bound = _attend(q[rows].view(hi - lo, hq, d), kc, ks, vc, vs, bt[b], lens[b],
+                                      past + torch.arange(lo, hi, device="cuda"), d ** -0.5, hkv)
+                _near(out[rows], want, bound, f"turn {turn}, {past} + {n}, rows {lo}..{hi}")
+
+
 def test_prefill_non_finite_and_errors(cuda):
     """A NaN block reaches only rows that see it; sequences outside the launch's sizes are
     latched and skipped, the others right."""
