@@ -821,7 +821,9 @@ __global__ void __launch_bounds__(G * WR * 32) prefill_fp8_kernel(const PrefillF
       for (int nt = 0; nt < 8; ++nt) {
         s[nt][2 * hr] = exp2f(s[nt][2 * hr] - m_use);
         s[nt][2 * hr + 1] = exp2f(s[nt][2 * hr + 1] - m_use);
-        sum = fmaf(s[nt][2 * hr] + s[nt][2 * hr + 1], s_scale[2][nt >> 1], sum);
+        // a block that this row does not see must not reach it even as NaN
+        if (t * kQpKeys + (nt >> 1) * kKvBlock <= (hr ? lim1 : lim0))
+          sum = fmaf(s[nt][2 * hr] + s[nt][2 * hr + 1], s_scale[2][nt >> 1], sum);
       }
       l_row[hr] = l_row[hr] * corr[hr] + sum;
     }
@@ -901,10 +903,13 @@ extern "C" size_t muk_decode_attn_fp8_workspace_size(int num_seqs, int num_q_hea
   if (num_seqs <= 0 || num_q_heads <= 0 || head_dim <= 0 || max_seq_len <= 0 ||
       block_size != kKvBlock)
     return 0;
-  // Batches of more than kQdFlatSeqs sequences need none, but a smaller one may follow.
+  // Batches of more than kQdFlatSeqs sequences need none, but a smaller one may follow, and
+  // a shorter longest context may have more partial results (its runs may be shorter).
   const int n = num_seqs < kQdFlatSeqs ? num_seqs : kQdFlatSeqs;
-  const DecodeFp8Plan p = decode_fp8_plan(max_seq_len, n);
-  return decode_fp8_workspace(n, num_q_heads, head_dim, p.max_parts);
+  const int most = ((max_seq_len - 1) / kKvBlock + 1) / kQdMinRun + 2;
+  const DecodeFp8Plan p = decode_fp8_plan(max_seq_len, 1);
+  return decode_fp8_workspace(n, num_q_heads, head_dim,
+                              p.max_parts == 0 ? 0 : most < kQdMaxParts ? most : kQdMaxParts);
 }
 
 extern "C" int muk_paged_decode_attn_fp8(const void* q, int64_t q_stride, void* out,

@@ -632,13 +632,15 @@ bool prefill_fp8_tc_supported(int head_dim, int num_q_heads, int num_kv_heads) {
 }
 
 int launch_prefill_fp8_tc(const PrefillFp8Args& a, int num_seqs, int max_q_len, cudaStream_t stream) {
+  const int P = 2 * kXRows / (a.num_q_heads / a.num_kv_heads);
+  MUK_REQUIRE((max_q_len + P - 1) / P <= 65535 && num_seqs <= 65535,
+              "muk_paged_prefill_attn_fp8: %d rows of a sequence", max_q_len);
   static std::atomic<uint64_t> attr_done{0};
   const cudaError_t ae = smem_attr_once(prefill_fp8_tc_kernel, XLayout::kBytes, attr_done);
   if (ae != cudaSuccess) {
     set_last_error("muk_paged_prefill_attn_fp8: cudaFuncSetAttribute: %s", cudaGetErrorString(ae));
     return MUK_ERR_CUDA;
   }
-  const int P = 2 * kXRows / (a.num_q_heads / a.num_kv_heads);
   launch_pdl(prefill_fp8_tc_kernel, dim3(a.num_kv_heads, (max_q_len + P - 1) / P, num_seqs),
              dim3(kXThreads), XLayout::kBytes, stream, a);
   return check_launch("muk_paged_prefill_attn_fp8");

@@ -67,9 +67,32 @@ def test_decode_refuses(change, code, text):
     (dict(d=32), -2, "head_dim"), (dict(ldo=516), -1, "strides"), (dict(out=OK + 8), -1, "strides"),
     (dict(scale=0.0), -1, "scale"), (dict(scale=float("nan")), -1, "scale"),
     (dict(max_len=130), -1, "block table"), (dict(nb=0), -1, "block table"),
-    (dict(B=70000), -1, "sequences")])
+    (dict(B=70000), -1, "sequences"), (dict(max_q=600000), -1, "rows of a sequence"),
+    (dict(hq=128, ldq=16384, ldo=16384, max_q=131072), -1, "rows of a sequence")])
 def test_prefill_refuses(change, code, text):
     _refused("muk_paged_prefill_attn_fp8", list({**PREFILL, **change}.values()), code, text)
+
+
+def test_decode_workspace_serves_smaller_batches():
+    """What a workspace was sized for covers fewer sequences and shorter contexts, each of
+    which the entry point may cut into other runs."""
+    lib = _lib()
+
+    def needs(n, length):  # as the entry point says when it has none
+        rc = lib.load().muk_paged_decode_attn_fp8(*{**DECODE, "B": n, "max_len": length,
+                                                    "bts": 1 << 20}.values())
+        return 0 if rc != -3 else int(lib.last_error().split(" bytes")[0].split()[-1])
+
+    def size(n, length):
+        return lib.load().muk_decode_attn_fp8_workspace_size(n, DECODE["hq"], DECODE["d"], length, 16)
+
+    lengths = [257, 300, 4096, 12000, 23999, 24000, 24001, 24016, 30000, 32768, 48000, 48001, 100000]
+    for i, length in enumerate(lengths):
+        for n in (1, 7, 2048, 4000):
+            for shorter in lengths[: i + 1]:
+                for fewer in (1, 5, 2048):
+                    if fewer <= n:
+                        assert 0 < needs(fewer, shorter) <= size(n, length), (n, length, fewer, shorter)
 
 
 @pytest.mark.parametrize("src,dst,change,text", [

@@ -152,6 +152,59 @@ def test_decode_batches(cuda, n, length):
         _near(outs[0][b:b + 1], want, bound, f"sequence {b} of {lens[b]}")
 
 
+@pytest.mark.parametrize("n,hq,hkv,d,length", [(2100, 4, 2, 64, 600), (70, 6, 6, 64, 900),
+                                               (40, 36, 12, 128, 1500), (33, 9, 3, 128, 2000),
+                                               (2048, 2, 1, 64, 300)])
+def test_decode_spreads(cuda, n, hq, hkv, d, length):
+    """More sequences than are cut into equal runs, head counts that leave groups of one,
+    two or four heads, blocks shared by several sequences."""
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, length + 1, (n,), generator=g).int()
+    lens[n // 2] = length
+    nb = 400
+    bt = torch.randint(0, nb, (n, (length + BS - 1) // BS), generator=g).int().cuda()
+    kc, ks = _quantised(nb, hkv, d, 31)
+    vc, vs = _quantised(nb, hkv, d, 32, spread=2.0)
+    q = torch.randn(n, hq * d, device="cuda", generator=_gen(8)).bfloat16()
+    out = torch.full_like(q, 7.0)
+    ws = torch.empty(max(4, _k().decode_attn_fp8_workspace_size(n, hq, d, length) // 4), device="cuda")
+    _k().decode_attn_fp8(q, out, kc, vc, ks, vs, bt, lens.cuda(), hq, hkv, d, length, workspace=ws)
+    assert _err() == 0
+    for b in list(range(0, n, max(1, n // 40))) + [n // 2, n - 1]:
+        ctx = int(lens[b])
+        if ctx == 0:
+            assert bool((out[b] == 0).all())
+            continue
+        want, bound = _attend(q[b:b + 1].view(1, hq, d), kc, ks, vc, vs, bt[b], ctx,
+                              torch.tensor([ctx - 1], device="cuda"), d ** -0.5, hkv)
+        _near(out[b:b + 1], want, bound, f"sequence {b} of {ctx}")
+
+
+def test_decode_workspace_of_a_longer_bound(cuda):
+    """A workspace sized for 24,016 tokens serves a launch of up to 24,000, which is cut
+    into shorter runs; two streams with workspaces of their own do not disturb each other."""
+    hq, hkv, d = 8, 2, 128
+    lens = [24000, 5, 17000]
+    bt, nb = _tables(lens, 77)
+    kc, ks = _quantised(nb, hkv, d, 33)
+    vc, vs = _quantised(nb, hkv, d, 34)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    size = _k().decode_attn_fp8_workspace_size(3, hq, d, 24016)
+    qs = [torch.randn(3, hq * d, device="cuda", generator=_gen(i)).bfloat16() for i in (9, 10)]
+    outs, wss = [torch.empty_like(q) for q in qs], [torch.empty(size // 4, device="cuda") for _ in qs]
+    torch.cuda.synchronize()
+    for q, out, ws, stream in zip(qs, outs, wss, (torch.cuda.Stream(), torch.cuda.Stream())):
+        with torch.cuda.stream(stream):
+            _k().decode_attn_fp8(q, out, kc, vc, ks, vs, bt, sl, hq, hkv, d, 24000, workspace=ws)
+    torch.cuda.synchronize()
+    assert _err() == 0
+    for q, out in zip(qs, outs):
+        for b, ctx in enumerate(lens):
+            want, bound = _attend(q[b:b + 1].view(1, hq, d), kc, ks, vc, vs, bt[b], ctx,
+                                  torch.tensor([ctx - 1], device="cuda"), d ** -0.5, hkv)
+            _near(out[b:b + 1], want, bound, f"sequence {b}")
+
+
 def test_decode_scales_and_non_finite(cuda):
     """Any positive scales, far apart; tiny and huge queries; a NaN block scale or a
     NaN query reaches its own heads and nothing else."""
@@ -258,6 +311,30 @@ def test_prefill_long(cuda, past, n, gain):
         want, bound = _attend(q[lo:hi].view(hi - lo, hq, d), kc, ks, vc, vs, bt[0], ctx,
                               past + torch.arange(lo, hi, device="cuda"), d ** -0.5, hkv)
         _near(outs[0][lo:hi], want, bound, f"rows {lo}..{hi}")
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (8, 2, 64), (6, 2, 128), (2, 2, 64)])
+def test_prefill_hidden_block_of_nan(cuda, hq, hkv, d):
+    """A block whose scale is NaN reaches the rows that see a key of it and no others, also
+    those whose 64-key tile holds it."""
+    n, at = 200, 9                                # keys 144..159 of the tile 128..191
+    bt, nb = _tables([n], 23)
+    kc, ks = _quantised(nb, hkv, d, 17)
+    vc, vs = _quantised(nb, hkv, d, 18)
+    bad = int(bt[0, at])
+    ks[bad, 0] = float("nan")
+    vs[bad, 1] = float("nan")
+    q = torch.randn(n, hq * d, device="cuda", generator=_gen(7)).bfloat16()
+    out = torch.zeros_like(q)
+    _k().prefill_attn_fp8(q, out, kc, vc, ks, vs, bt, torch.tensor([n], dtype=torch.int32, device="cuda"),
+                          torch.tensor([0, n], dtype=torch.int32, device="cuda"), n, hq, hkv, d)
+    assert _err() == 0
+    assert bool(out[16 * at:].isnan().all()) and not bool(out[:16 * at].isnan().any())
+    rows = slice(130, 16 * at)
+    ks[bad] = vs[bad] = 1.0
+    want, bound = _attend(q[rows].view(-1, hq, d), kc, ks, vc, vs, bt[0], n,
+                          torch.arange(130, 16 * at, device="cuda"), d ** -0.5, hkv)
+    _near(out[rows], want, bound, "rows before the block")
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (16, 2, 128), (8, 4, 64)])
