@@ -182,28 +182,40 @@ def prefill_attn(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_ca
 # 8-bit KV cache: e4m3 codes [num_blocks, Hkv, 16, D] and one f32 scale for each
 # (block, head), [num_blocks, Hkv]; a cached value is code * scale.
 # ---------------------------------------------------------------------------
-def _check_here(name: str, *tensors: torch.Tensor | None) -> None:
-    """Every tensor on the current CUDA device: the launch goes to its stream."""
-    dev = torch.cuda.current_device()
+# The 8-bit entry points check every argument.  A decode step's call is over in ~6 us on the
+# device, so the checks read each attribute once (size(i) and stride(i) take longer than
+# shape and stride()).
+_FP8, _BF16, _F32, _I32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.int32
+
+
+def _check_here(name: str, first: torch.Tensor, *tensors: torch.Tensor | None) -> int:
+    """The current stream; every tensor has to be on the current CUDA device, whose stream
+    the launch goes to."""
+    dev = first.get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
-            raise ValueError(f"{name}: every tensor must be on the current CUDA device (cuda:{dev}), "
-                             f"got one on {t.device}")
+            raise ValueError(f"{name}: every tensor must be on the current CUDA device, got one on "
+                             f"{first.device} and one on {t.device}")
+    if dev < 0 or dev != torch.cuda.current_device():
+        raise ValueError(f"{name}: every tensor must be on the current CUDA device, got one on "
+                         f"{first.device}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _check_cache_fp8(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                      v_scale: torch.Tensor, num_kv_heads: int, head_dim: int) -> tuple[int, int]:
     """(num_blocks, block_size) of a layer's 8-bit cache, its types and shapes checked."""
-    shape = k_cache.shape
-    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != torch.float8_e4m3fn:
+    if k_cache.dtype is not _FP8 or v_cache.dtype is not _FP8:
         raise TypeError(f"{name}: expected float8_e4m3fn caches, got {k_cache.dtype} / {v_cache.dtype}")
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+    if k_scale.dtype is not _F32 or v_scale.dtype is not _F32:
         raise TypeError(f"{name}: expected float32 scales, got {k_scale.dtype} / {v_scale.dtype}")
+    shape = k_cache.shape
     if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != head_dim or v_cache.shape != shape:
         raise ValueError(f"{name}: caches must be [num_blocks, {num_kv_heads}, block_size, {head_dim}], "
                          f"got {tuple(shape)} / {tuple(v_cache.shape)}")
-    if k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
-        raise ValueError(f"{name}: scales must be {tuple(shape[:2])}, got {tuple(k_scale.shape)} / "
+    blocks = (shape[0], num_kv_heads)
+    if k_scale.shape != blocks or v_scale.shape != blocks:
+        raise ValueError(f"{name}: scales must be {blocks}, got {tuple(k_scale.shape)} / "
                          f"{tuple(v_scale.shape)}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
             and v_scale.is_contiguous()):
@@ -212,26 +224,37 @@ def _check_cache_fp8(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, k_
 
 
 def _check_index(name: str, t: torch.Tensor, what: str, at_least: int) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.stride(0) != 1 or t.shape[0] < at_least:
+    shape = t.shape
+    if t.dtype is not _I32 or len(shape) != 1 or shape[0] < at_least or not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous int32 with at least {at_least} entries, "
-                         f"got {t.dtype} {tuple(t.shape)}")
+                         f"got {t.dtype} {tuple(shape)}")
 
 
 def _check_rows(name: str, t: torch.Tensor, what: str, rows: int, width: int) -> int:
     """Row stride of a [rows.., width..] bf16 tensor."""
-    if t.dtype != torch.bfloat16:
+    if t.dtype is not _BF16:
         raise TypeError(f"{name}: {what} must be bfloat16, got {t.dtype}")
-    if t.dim() != 2 or t.stride(1) != 1 or t.shape[0] < rows or t.shape[1] < width:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or strides[1] != 1 or shape[0] < rows or shape[1] < width:
         raise ValueError(f"{name}: {what} must be [>= {rows}, >= {width}] with contiguous rows, got "
-                         f"{tuple(t.shape)}")
-    return t.stride(0)
+                         f"{tuple(shape)}")
+    return strides[0]
 
 
-def _check_tables(name: str, bt: torch.Tensor, rows: int) -> int:
-    if bt.dtype != torch.int32 or bt.dim() != 2 or bt.stride(1) != 1 or bt.shape[0] < rows:
+def _check_tables(name: str, bt: torch.Tensor, rows: int, block_size: int,
+                  max_seq_len: int | None) -> tuple[int, int]:
+    """(row stride, longest context: max_seq_len or what a row holds) of block tables."""
+    shape, strides = bt.shape, bt.stride()
+    if bt.dtype is not _I32 or len(shape) != 2 or strides[1] != 1 or shape[0] < rows:
         raise ValueError(f"{name}: block_tables must be int32 [>= {rows}, blocks] with contiguous rows, "
-                         f"got {bt.dtype} {tuple(bt.shape)}")
-    return bt.shape[1] if bt.shape[0] <= 1 else bt.stride(0)
+                         f"got {bt.dtype} {tuple(shape)}")
+    room = shape[1] * block_size
+    if max_seq_len is None:
+        max_seq_len = room
+    elif room < max_seq_len:
+        raise ValueError(f"{name}: block_tables hold {shape[1]} blocks, max_seq_len {max_seq_len} "
+                         "needs more")
+    return (shape[1] if shape[0] <= 1 else strides[0]), max_seq_len
 
 
 def rope_kv_append_fp8(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
@@ -254,22 +277,23 @@ def rope_kv_append_fp8(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping:
     ldq = _check_rows(name, q, "q_out", T, num_q_heads * head_dim)
     _check_index(name, positions, "positions", T)
     _check_index(name, slot_mapping, "slot_mapping", T)
-    for t in (rope_cos, rope_sin):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != head_dim // 2 \
-                or not t.is_contiguous() or t.shape[0] != rope_cos.shape[0]:
-            raise ValueError(f"{name}: RoPE tables must be contiguous float32 [positions, "
-                             f"{head_dim // 2}]")
+    table = rope_cos.shape
+    if rope_cos.dtype is not _F32 or rope_sin.dtype is not _F32 or len(table) != 2 \
+            or table[1] != head_dim // 2 or rope_sin.shape != table \
+            or not (rope_cos.is_contiguous() and rope_sin.is_contiguous()):
+        raise ValueError(f"{name}: RoPE tables must be contiguous float32 [positions, "
+                         f"{head_dim // 2}]")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != head_dim
+        if w is not None and (w.dtype is not _F32 or w.numel() != head_dim
                               or not w.is_contiguous()):
             raise ValueError(f"{name}: norm weights must be contiguous float32 [{head_dim}]")
-    _check_here(name, qkv, q, positions, slot_mapping, rope_cos, rope_sin, k_cache, v_cache,
-                k_scale, v_scale, q_norm_w, k_norm_w)
+    stream = _check_here(name, qkv, q, positions, slot_mapping, rope_cos, rope_sin, k_cache, v_cache,
+                         k_scale, v_scale, q_norm_w, k_norm_w)
     call("muk_rope_kv_append_fp8", qkv.data_ptr(), ld, q.data_ptr(), ldq, positions.data_ptr(),
-         slot_mapping.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], T,
+         slot_mapping.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), table[0], T,
          num_q_heads, num_kv_heads, head_dim, _p(q_norm_w), _p(k_norm_w), qk_eps,
          k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-         num_blocks, block_size, _stream())
+         num_blocks, block_size, stream)
 
 
 def decode_attn_fp8_workspace_size(num_seqs: int, num_q_heads: int, head_dim: int,
@@ -293,19 +317,17 @@ def decode_attn_fp8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     B = seq_lens.shape[0] if num_seqs is None else num_seqs
     ldq = _check_rows(name, q, "q", B, num_q_heads * head_dim)
     ldo = _check_rows(name, out, "out", B, num_q_heads * head_dim)
-    bts = _check_tables(name, block_tables, B)
-    if block_tables.shape[1] * block_size < max_seq_len:
-        raise ValueError(f"{name}: block_tables hold {block_tables.shape[1]} blocks, max_seq_len "
-                         f"{max_seq_len} needs more")
+    bts, _ = _check_tables(name, block_tables, B, block_size, max_seq_len)
     _check_index(name, seq_lens, "seq_lens", B)
-    _check_here(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, workspace)
+    stream = _check_here(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
+                         workspace)
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError(f"{name}: workspace must be contiguous")
     call("muk_paged_decode_attn_fp8", q.data_ptr(), ldq, out.data_ptr(), ldo, k_cache.data_ptr(),
          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), bts,
          seq_lens.data_ptr(), B, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
          head_dim ** -0.5 if scale is None else scale, max_seq_len, _p(workspace),
-         0 if workspace is None else workspace.nbytes, _stream())
+         0 if workspace is None else workspace.nbytes, stream)
 
 
 def prefill_attn_fp8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
@@ -323,22 +345,16 @@ def prefill_attn_fp8(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor,
     B = seq_lens.shape[0] if num_seqs is None else num_seqs
     ldq = _check_rows(name, q, "q", 0, num_q_heads * head_dim)
     ldo = _check_rows(name, out, "out", 0, num_q_heads * head_dim)
-    bts = _check_tables(name, block_tables, B)
-    room = block_tables.shape[1] * block_size
-    if max_seq_len is None:
-        max_seq_len = room
-    elif room < max_seq_len:
-        raise ValueError(f"{name}: block_tables hold {block_tables.shape[1]} blocks, max_seq_len "
-                         f"{max_seq_len} needs more")
+    bts, max_seq_len = _check_tables(name, block_tables, B, block_size, max_seq_len)
     _check_index(name, seq_lens, "seq_lens", B)
     _check_index(name, cu_seqlens_q, "cu_seqlens_q", B + 1)
-    _check_here(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
-                cu_seqlens_q)
+    stream = _check_here(name, q, out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
+                         cu_seqlens_q)
     call("muk_paged_prefill_attn_fp8", q.data_ptr(), ldq, out.data_ptr(), ldo, k_cache.data_ptr(),
          v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), bts,
          seq_lens.data_ptr(), cu_seqlens_q.data_ptr(), B, min(q.shape[0], out.shape[0]), max_q_len,
          max_seq_len, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks,
-         head_dim ** -0.5 if scale is None else scale, _stream())
+         head_dim ** -0.5 if scale is None else scale, stream)
 
 
 def copy_pages(pool: torch.Tensor, src: Sequence[int], dst: Sequence[int],
@@ -362,12 +378,12 @@ def copy_pages(pool: torch.Tensor, src: Sequence[int], dst: Sequence[int],
     s, d = array.array("i", src), array.array("i", dst)
     if len(s) != len(d):
         raise ValueError(f"{name}: {len(s)} sources for {len(d)} destinations")
-    _check_here(name, pool, scales)
+    stream = _check_here(name, pool, scales)
     if len(s) == 0:
         return
     _lib.call_counted("muk_copy_pages", (len(s) + 255) // 256, pool.data_ptr(), num_blocks * page,
                       planes, page, _p(scales), num_blocks * sbytes, sbytes, num_blocks,
-                      s.buffer_info()[0], d.buffer_info()[0], len(s), _stream())
+                      s.buffer_info()[0], d.buffer_info()[0], len(s), stream)
 
 
 def gemm(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, epilogue: int = MUK_EPI_BF16,
