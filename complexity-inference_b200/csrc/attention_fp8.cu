@@ -1040,6 +1040,7 @@ extern "C" int muk_paged_prefill_attn_fp8(const void* q, int64_t q_stride, void*
   a.num_kv_heads = num_kv_heads;
   a.num_blocks = num_blocks;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.splits = 1;
   cudaStream_t s = as_stream(stream);
   if (prefill_fp8_tc_supported(head_dim, num_q_heads, num_kv_heads))
     return launch_prefill_fp8_tc(a, num_seqs, max_q_len, s);

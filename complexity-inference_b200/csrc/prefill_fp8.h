@@ -23,11 +23,12 @@ struct PrefillFp8Args {
   int num_q_heads, num_kv_heads, num_blocks;
   int num_rows, max_q_len, max_blocks;
   float scale_log2;
+  int splits;  // CTAs of a cluster that share the keys of a query tile (tensor-memory kernel)
 };
 
 // True for the shapes of the tensor-memory kernel: head_dim 128 and a group that
 // divides its 128-row tile.
 bool prefill_fp8_tc_supported(int head_dim, int num_q_heads, int num_kv_heads);
-int launch_prefill_fp8_tc(const PrefillFp8Args& a, int num_seqs, int max_q_len, cudaStream_t stream);
+int launch_prefill_fp8_tc(PrefillFp8Args a, int num_seqs, int max_q_len, cudaStream_t stream);
 
 }  // namespace muk

@@ -31,6 +31,13 @@
 // stay below 2^8 and O is rescaled in TMEM on those tiles alone (after P V of the
 // tile before has run); O and l use the same bound.
 //
+// Few rows, long contexts (a short chunk behind a long past): where the query tiles would
+// fill less than half of the SMs, the CTAs of a cluster of 2, 4 or 8 share the keys of one,
+// at least 8 tiles each, and join their (m, l, O) through distributed shared memory, every
+// CTA finishing a part of the rows.  64 rows behind 32k tokens (32 heads) took 566 us in one
+// CTA per tile and take 95, one row behind 8k 144 and 37; with at least 16 tiles each, 64
+// rows behind 1k took 28 us for 23.
+//
 // Every wait is bounded (common.cuh); on time-out the kernel records the error
 // word, every role leaves its loop, TMEM is freed and the CTA returns.
 #include <math.h>
@@ -60,6 +67,8 @@ constexpr int kXItem = kXKeys * 128; // bytes of such a tile
 // constants older than those of tile t - kXRing - kXStages + 1.
 constexpr int kXConsts = 16;
 static_assert(kXConsts > kXRing + kXStages + 2, "block constants are overwritten in use");
+constexpr int kXSplits = 8;          // CTAs that share the keys of a query tile, at most
+constexpr int kXSplitTiles = 8;      // key tiles of each, at least
 constexpr int kXQPanel = 128 * 128;  // [128 rows][64 f16], one swizzled panel of a query tile
 constexpr int kXPanel = kXKeys * 128;  // the same of a K or V tile
 
@@ -74,6 +83,9 @@ struct XLayout {
   static constexpr int kBytes = kScale + kXConsts * 4 * 16 + 1024;  // + alignment slack
 };
 static_assert(XLayout::kBytes <= 232448, "prefill tile exceeds 227 KB of shared memory");
+static_assert((kXSplits - 1) * (2 * kXRows / kXSplits) * (kXD * 4 + 8) <= XLayout::kBar - XLayout::kK,
+              "the rows of a join exceed the tiles' memory");
+static_assert(kXSplitTiles >= kXSplits, "a CTA of a cluster could be left without tiles");
 
 // Bounded wait of a whole warp (about a second).  One try on a complete barrier is
 // ~110 clocks, so roles keep few barriers; the polls are one loop in PTX (as a C++ loop
@@ -208,12 +220,21 @@ __device__ __forceinline__ void x_tmem_st16(uint32_t taddr, const uint32_t (&r)[
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// An address of this CTA's shared memory as that of the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t x_mapa(uint32_t addr, int rank) {
+  uint32_t y;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(addr), "r"(rank));
+  return y;
+}
 // Instruction descriptor, kind::f16: f16 A/B (format 0), f32 D, A K-major.
 __host__ __device__ constexpr uint32_t x_idesc(bool b_mn, int n) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kXRows >> 4) << 24);
 }
 
+// Split: the CTAs of a cluster share a query tile's keys (otherwise one has all of them, in
+// code without the join: as one kernel for both, 4,000 tokens took 172 us for 164).
+template <bool Split>
 __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const PrefillFp8Args a) {
   // programmatic dependent launch: let the next kernel launch once every CTA
   // of this one runs, and wait for the previous kernel before touching memory
@@ -236,7 +257,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z, kvh = blockIdx.x;
+  const int b = blockIdx.z, kvh = Split ? blockIdx.x / a.splits : blockIdx.x;
   const int qt = (int)gridDim.y - 1 - (int)blockIdx.y;  // longest (last) query tiles first
   const int G = a.num_q_heads / a.num_kv_heads;
   const int P = 2 * kXRows / G;                          // positions of the CTA
@@ -256,6 +277,15 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     return;
   }
   const int32_t* bt = a.block_tables + (int64_t)b * a.bt_stride;
+  // The key tiles are shared out over the CTAs of a cluster, as many as get kXSplitTiles
+  // each (all of a cluster come to the same number); this one has tiles t0 .. t0 + nl - 1.
+  int splits = Split ? a.splits : 1;
+  while (Split && splits > 1 && nt < kXSplitTiles * splits) splits >>= 1;
+  const int rank = Split ? (int)blockIdx.x % a.splits : 0;
+  const int per = Split ? (nt + splits - 1) / splits : nt;
+  const int t0 = Split ? rank * per : 0;
+  const int nl = Split ? min(per, nt - t0) : nt;         // > 0 for rank < splits: nt >= splits^2
+  if (Split && rank >= splits) return;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kXStages; ++i) {
@@ -287,6 +317,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  float m_used = -INFINITY, l = 0.f;  // of a softmax thread's row
 
   if (warp == kXIssuer || warp == kXIssuer1) {
     // ---- MMA issuers ---------------------------------------------------------
@@ -317,19 +348,19 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
                  x_idesc(true, kXD), (t > 0 || k > 0) ? 1u : 0u);
       // a barrier of its own for the last one: its reader may be two tiles ahead of the
       // multiplies there, which the phase of o_done cannot tell
-      x_commit(lead, t + 1 < nt ? &o_done[qi] : &o_last[qi]);
+      x_commit(lead, t + 1 < nl ? &o_done[qi] : &o_last[qi]);
     };
-    // Step t = -2 .. nt - 1 uses V(t) and K(t + 2) of stage (t + 2) % kXStages.
+    // Step t = -2 .. nl - 1 uses V(t) and K(t + 2) of stage (t + 2) % kXStages.
     bool ok = x_wait(q_full, 0, kDevTimeoutFull);
     int sg = 0;
     uint32_t ph = 0;
-    for (int t = -2; ok && t < nt; ++t) {
+    for (int t = -2; ok && t < nl; ++t) {
       ok = x_wait(&st_full[sg], ph, kDevTimeoutFull);
       if (ok && t >= 0) ok = x_wait(&p_full[qi * 2 + (t & 1)], (uint32_t)(t >> 1) & 1u, kDevTimeoutFull);
       if (!ok) break;
       tc_fence_after();
       if (t >= 0) pv(t, sg);
-      if (t + 2 < nt) qk(t + 2, sg);
+      if (t + 2 < nl) qk(t + 2, sg);
       x_commit(lead, &st_empty[sg]);
       if (++sg == kXStages) sg = 0, ph ^= 1;
     }
@@ -349,9 +380,11 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     const uint8_t* src = (mine_k ? a.k_cache : a.v_cache) + (int64_t)kvh * (kKvBlock * kXD);
     const int64_t blk_bytes = (int64_t)a.num_kv_heads * (kKvBlock * kXD);
     const uint32_t dst = base + (uint32_t)(XLayout::kRaw + (mine_k ? kXItem : 0) + (lane & 3) * 2048);
+    const int mine_blks = min(nl * 4, nblk - t0 * 4);  // of this CTA's tiles
     auto block_of = [&](int t) {                     // of this lane in step t, -1: none
       const int blk = (mine_k ? t + 2 : t) * 4 + (lane & 3);
-      return lane < 8 && blk >= 0 && blk < nblk ? blk : -1;
+      if (!Split) return lane < 8 && blk >= 0 && blk < nblk ? blk : -1;
+      return lane < 8 && blk >= 0 && blk < mine_blks ? t0 * 4 + blk : -1;
     };
     auto id_of = [&](int t) {
       const int blk = block_of(t);
@@ -366,7 +399,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     int id = id_of(-2), id_next = id_of(-1), slot = 0, issued = 0;
     float2 scales = scales_of(-2, id);
     uint32_t ph = 1;
-    for (int t = -2; t < nt; ++t) {
+    for (int t = -2; t < nl; ++t) {
       if (!x_wait(raw_empty + slot, ph, kDevTimeoutEmpty)) break;
       const bool have = block_of(t) >= 0;
       const int blocks = __popc(__ballot_sync(0xffffffffu, have));
@@ -382,7 +415,7 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
                 dst + (uint32_t)(slot * 2 * kXItem)),
             "l"(src + id * blk_bytes), "r"(smem_u32(raw_full + slot))
             : "memory");
-      if (mine_k && lane < 8 && t + 2 < nt) {
+      if (mine_k && lane < 8 && t + 2 < nl) {
         const float ks = clamp_scale(scales.x), vs = clamp_scale(scales.y);
         float lv, iv;
         asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(vs));  // exact for powers of two
@@ -423,10 +456,10 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       }
     };
     auto convert = [&](uint4 (&v)[kBpt], int t, uint32_t at) {
-      if (t == nt - 1) {  // rows behind the last key are zero: what the blocks hold there is not ours
+      if (t0 + t == nt - 1) {  // rows behind the last key are zero: what the blocks hold there is not ours
 #pragma unroll
         for (int j = 0; j < kBpt; ++j)
-          if (t * kXKeys + j * kKvBlock + row >= n_keys) v[j] = make_uint4(0u, 0u, 0u, 0u);
+          if ((t0 + t) * kXKeys + j * kKvBlock + row >= n_keys) v[j] = make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
       for (int j = 0; j < kBpt; ++j) {
@@ -444,8 +477,8 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     };
     int slot = 0, sg = 0;
     uint32_t ph_r = 0, ph = 1;                       // parities: ring "full", stage "empty"
-    for (int t = -2; t < nt; ++t) {                  // step t: V(t) and K(t + 2)
-      const bool has_v = t >= 0, has_k = t + 2 < nt;
+    for (int t = -2; t < nl; ++t) {                  // step t: V(t) and K(t + 2)
+      const bool has_v = t >= 0, has_k = t + 2 < nl;
       uint4 vv[kBpt], vk[kBpt];
       if (!x_wait(raw_full + slot, ph_r, kDevTimeoutFull)) break;
       const uint32_t src = ring + (uint32_t)(slot * 2 * kXItem);
@@ -511,15 +544,14 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       if (lane == 0) mbar_arrive(q_full);
     }
     const float4* consts = reinterpret_cast<const float4*>(basep + XLayout::kScale);
-    float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int t = 0; t < nt; ++t) {
+    for (int t = 0; t < nl; ++t) {
       const int sb = qi * 2 + (t & 1);
       const uint32_t ts = lane_base + (uint32_t)(sb * kXKeys);
       ok = x_wait(&s_full[sb], (uint32_t)(t >> 1) & 1u, kDevTimeoutAccum);
       if (!ok) break;
       tc_fence_after();
-      const int k0 = t * kXKeys;
+      const int k0 = (t0 + t) * kXKeys;
       const bool diagonal = k0 + kXKeys - 1 > tile_limit;  // uniform: some row's limit falls in the tile
       const float4* cs = consts + (t % kXConsts) * 4;
       uint32_t s[2][32];
@@ -593,7 +625,8 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
       if (lane == 0) mbar_arrive(&p_full[sb]);
     }
     if (ok) ok = x_wait(&o_last[qi], 0, kDevTimeoutAccum);
-    if (ok) {
+    if (Split && splits > 1 && !ok) m_used = -INFINITY, l = 0.f;  // nothing to join
+    if (ok && (!Split || splits == 1)) {
       tc_fence_after();
       const float inv = 1.f / l;
       uint4* dst = reinterpret_cast<uint4*>(
@@ -618,6 +651,99 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
     }
   }
 
+  if (Split && splits > 1) {
+    // ---- join of the cluster's results (m, l, O): a CTA finishes the rows of 8 / splits
+    // softmax warps, the others write theirs into its memory over the tiles
+    tc_fence_before();
+    cluster_sync();  // every CTA is done with its tiles
+    tc_fence_after();
+    const int warps = 8 / splits, owner = warp / warps;
+    const uint32_t rows = (uint32_t)warps * 32;
+    const uint32_t box = base + (uint32_t)XLayout::kK;                   // [sender][row][128] f32
+    const uint32_t ml = box + (uint32_t)(splits - 1) * rows * (kXD * 4); // [sender][row] (m, l)
+    const uint32_t my = (uint32_t)(warp % warps) * 32 + lane;            // this thread's row there
+    const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) +
+                        (uint32_t)(4 * kXKeys + (warp >> 2) * kXD);
+    // 16-byte chunk c of a row lies at c ^ lane, or 32 rows would meet in four banks
+    uint32_t rr[32];
+    if (warp < 8 && owner != rank) {
+      const uint32_t at = (uint32_t)(rank < owner ? rank : rank - 1) * rows + my;
+      const uint32_t dst = x_mapa(box + at * (kXD * 4), owner), dml = x_mapa(ml + at * 8, owner);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        tmem_ld_32x32b_x32(to + 32 * i, rr);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
+                           dst + (uint32_t)(((i * 8 + j) ^ lane) << 4)),
+                       "r"(rr[4 * j]), "r"(rr[4 * j + 1]), "r"(rr[4 * j + 2]), "r"(rr[4 * j + 3])
+                       : "memory");
+      }
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(dml), "f"(m_used), "f"(l)
+                   : "memory");
+    }
+    cluster_sync();  // the rows have arrived; from here on a CTA reads its own memory only
+    if (warp < 8 && owner == rank) {
+      const int row = warp * 32 + lane, pos = p0 + row / G, h = kvh * G + row % G;
+      auto get_ml = [&](int s, float& m, float& x) {
+        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(m), "=f"(x) : "r"(ml + (s * rows + my) * 8) : "memory");
+      };
+      float M = m_used;
+      for (int s = 0; s < splits - 1; ++s) {
+        float m, x;
+        get_ml(s, m, x);
+        M = fmaxf(M, m);
+      }
+      // a row without a bound has seen no key (l 0), or NaN alone
+      auto factor = [&](float m, float x) {
+        return m == -INFINITY ? (x != 0.f ? 1.f : 0.f) : x_exp2(m - M);
+      };
+      const float own = factor(m_used, l);
+      float L = own != 0.f ? own * l : 0.f;
+      for (int s = 0; s < splits - 1; ++s) {
+        float m, x;
+        get_ml(s, m, x);
+        const float f = factor(m, x);
+        if (f != 0.f) L = fmaf(f, x, L);
+      }
+      const float inv = 1.f / L;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        tmem_ld_32x32b_x32(to + 32 * i, rr);
+        tmem_ld_wait();
+        float o[32];
+#pragma unroll
+        for (int u = 0; u < 32; ++u) o[u] = own != 0.f ? own * __uint_as_float(rr[u]) : 0.f;
+        for (int s = 0; s < splits - 1; ++s) {
+          float m, x;
+          get_ml(s, m, x);
+          const float f = factor(m, x);
+          if (f != 0.f) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 v = ld_shared_f4(box + (s * rows + my) * (kXD * 4) + (uint32_t)(((i * 8 + j) ^ lane) << 4));
+              o[4 * j] = fmaf(f, v.x, o[4 * j]);
+              o[4 * j + 1] = fmaf(f, v.y, o[4 * j + 1]);
+              o[4 * j + 2] = fmaf(f, v.z, o[4 * j + 2]);
+              o[4 * j + 3] = fmaf(f, v.w, o[4 * j + 3]);
+            }
+          }
+        }
+        if (pos < q_len) {
+          uint4* dst = reinterpret_cast<uint4*>(a.out + (int64_t)(q_begin + pos) * a.out_stride +
+                                                (int64_t)h * kXD) + i * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            dst[j] = make_uint4(pack_bf16x2(o[8 * j] * inv, o[8 * j + 1] * inv),
+                                pack_bf16x2(o[8 * j + 2] * inv, o[8 * j + 3] * inv),
+                                pack_bf16x2(o[8 * j + 4] * inv, o[8 * j + 5] * inv),
+                                pack_bf16x2(o[8 * j + 6] * inv, o[8 * j + 7] * inv));
+        }
+      }
+    }
+  }
+
   tc_fence_before();
   __syncthreads();
   if (warp == kXIssuer) {
@@ -626,23 +752,65 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
   }
 }
 
+static int x_sm_count() {
+  static std::atomic<int> count[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if ((n = count[dev].load(std::memory_order_relaxed)) == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    count[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 bool prefill_fp8_tc_supported(int head_dim, int num_q_heads, int num_kv_heads) {
   const int G = num_q_heads / num_kv_heads;
   return head_dim == kXD && kXRows % G == 0;
 }
 
-int launch_prefill_fp8_tc(const PrefillFp8Args& a, int num_seqs, int max_q_len, cudaStream_t stream) {
+int launch_prefill_fp8_tc(PrefillFp8Args a, int num_seqs, int max_q_len, cudaStream_t stream) {
   const int P = 2 * kXRows / (a.num_q_heads / a.num_kv_heads);
   MUK_REQUIRE((max_q_len + P - 1) / P <= 65535 && num_seqs <= 65535,
               "muk_paged_prefill_attn_fp8: %d rows of a sequence", max_q_len);
-  static std::atomic<uint64_t> attr_done{0};
-  const cudaError_t ae = smem_attr_once(prefill_fp8_tc_kernel, XLayout::kBytes, attr_done);
+  const int qtiles = (max_q_len + P - 1) / P;
+  const int64_t ctas = (int64_t)a.num_kv_heads * qtiles * num_seqs;
+  const int64_t tiles = ((int64_t)a.max_blocks * kKvBlock + kXKeys - 1) / kXKeys;
+  a.splits = 1;
+  while (a.splits < kXSplits && ctas * a.splits * 2 <= x_sm_count() &&
+         tiles >= (int64_t)kXSplitTiles * a.splits * 2)
+    a.splits *= 2;
+  auto kernel = a.splits > 1 ? prefill_fp8_tc_kernel<true> : prefill_fp8_tc_kernel<false>;
+  static std::atomic<uint64_t> attr_done[2];
+  const cudaError_t ae = smem_attr_once(kernel, XLayout::kBytes, attr_done[a.splits > 1]);
   if (ae != cudaSuccess) {
     set_last_error("muk_paged_prefill_attn_fp8: cudaFuncSetAttribute: %s", cudaGetErrorString(ae));
     return MUK_ERR_CUDA;
   }
-  launch_pdl(prefill_fp8_tc_kernel, dim3(a.num_kv_heads, (max_q_len + P - 1) / P, num_seqs),
-             dim3(kXThreads), XLayout::kBytes, stream, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.num_kv_heads * a.splits), (unsigned)qtiles, (unsigned)num_seqs);
+  cfg.blockDim = dim3(kXThreads);
+  cfg.dynamicSmemBytes = XLayout::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.splits > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)a.splits;
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  const cudaError_t le = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (le != cudaSuccess) {
+    cudaGetLastError();
+    set_last_error("muk_paged_prefill_attn_fp8: launch failed: %s", cudaGetErrorString(le));
+    return MUK_ERR_CUDA;
+  }
   return check_launch("muk_paged_prefill_attn_fp8");
 }
 

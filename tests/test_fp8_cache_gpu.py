@@ -313,6 +313,47 @@ def test_prefill_long(cuda, past, n, gain):
         _near(outs[0][lo:hi], want, bound, f"rows {lo}..{hi}")
 
 
+@pytest.mark.parametrize("hq,hkv,cases", [
+    (4, 1, [(9000, 40), (600, 7), (1000, 1), (0, 5), (2500, 64)]),
+    (2, 2, [(3844, 256), (4095, 1), (5000, 200)]),
+    (16, 4, [(8000, 130), (511, 1), (1024, 64), (30000, 2)])])
+def test_prefill_few_rows_long_contexts(cuda, hq, hkv, cases):
+    """Launches whose key tiles are shared out over the CTAs of a cluster, each sequence
+    over as many as its context is long enough for; rows that see no key of the last share;
+    a NaN row and a NaN block reach nothing else; two runs agree bit for bit."""
+    d = 128
+    lens, qn = [p + n for p, n in cases], [n for _, n in cases]
+    cu = [0]
+    for n in qn:
+        cu.append(cu[-1] + n)
+    bt, nb = _tables(lens, hq)
+    kc, ks = _quantised(nb, hkv, d, 61, spread=1.0)
+    vc, vs = _quantised(nb, hkv, d, 62, spread=3.0)
+    q = torch.randn(cu[-1], hq * d, device="cuda", generator=_gen(63)).bfloat16()
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cud = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    outs = []
+    for _ in range(2):
+        out = torch.full_like(q, 7.0)
+        _k().prefill_attn_fp8(q, out, kc, vc, ks, vs, bt, sl, cud, max(qn), hq, hkv, d)
+        outs.append(out)
+    assert _err() == 0 and torch.equal(outs[0], outs[1])
+    for b, (past, n) in enumerate(cases):
+        for lo in range(0, n, 64):
+            hi = min(lo + 64, n)
+            rows = slice(cu[b] + lo, cu[b] + hi)
+            want, bound = _attend(q[rows].view(hi - lo, hq, d), kc, ks, vc, vs, bt[b], lens[b],
+                                  past + torch.arange(lo, hi, device="cuda"), d ** -0.5, hkv)
+            _near(outs[0][rows], want, bound, f"{past} + {n}, rows {lo}..{hi}")
+    q[cu[1] - 1] = float("nan")                      # the first sequence's last row
+    vs[int(bt[-1, 3])] = float("nan")                # all rows of the last one see it
+    _k().prefill_attn_fp8(q, out, kc, vc, ks, vs, bt, sl, cud, max(qn), hq, hkv, d)
+    nan = out.isnan()
+    assert bool(nan[cu[1] - 1].all()) and bool(nan[cu[-2]:].all())
+    nan[cu[1] - 1] = False
+    assert not bool(nan[:cu[-2]].any()) and _err() == 0
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(4, 2, 64), (8, 2, 64), (6, 2, 128), (2, 2, 64)])
 def test_prefill_hidden_block_of_nan(cuda, hq, hkv, d):
     """A block whose scale is NaN reaches the rows that see a key of it and no others, also
