@@ -26,13 +26,20 @@
 // tokens), or there are more than 2,048 of them, a warp takes whole pairs and nothing is
 // joined.
 //
+// Measured (32 query heads on 8, head_dim 128): 256 sequences of 200 to 1,500 tokens 90 us
+// (4.9 TB/s; floor 68), 32 of up to 32k 196 us (5.8 TB/s; floor 171; ~206 once the power cap
+// lowers the clock).  What bounds it now is the warps' chains of conversion, mma.sync and
+// exponentials, two warps per SM sub-partition: the same copies without them take 169 us as
+// 16 KB pieces.  Tried: such pieces by tensor copies from a loading warp 200 us, 2 KB tensor
+// copies per warp 221, four blocks ahead 200, 12 or 16 warps of fewer registers 201 to 216.
+//
 // Fragments: ldmatrix (plain for K, transposed for V) on 8-bit rows hands each lane four
 // neighbouring codes; the k (for V: m) index inside an MMA is a free permutation, chosen
 // so that those four codes are what the lane needs.
 //
 // Prefill (mma.sync, head_dim 64 and groups that the tensor-memory kernel does
 // not take): 64-key tiles staged as f16, rows masked causally at absolute
-// positions, the same weights w.
+// positions, the same weights w.  Three short prompts of a tiny model take 6.4 us.
 //
 // Semantics follow mu_inference/models/layers.py:700-723, as in attention.cu.
 #include <math.h>
@@ -47,7 +54,9 @@ namespace muk {
 constexpr int kQdWarps = 8;        // warps per decode CTA, one CTA per SM
 constexpr int kQdAhead = 2;        // blocks on their way, per warp
 constexpr int kQdStages = 2 + kQdAhead;  // cp.async ring per warp: two more in work
-constexpr int kQdMinRun = 12;      // blocks of a run, at least
+// Blocks of a run, at least: a shorter one costs more in its pair's join than it saves
+// (and a pair's partial results stay within kQdMaxParts).
+constexpr int kQdMinRun = 12;
 constexpr int kQdMaxParts = 127;   // partial results of a pair, at most
 constexpr int kQdFlatSeqs = 2048;  // sequences whose block counts a CTA adds up
 

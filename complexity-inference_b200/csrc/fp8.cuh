@@ -5,8 +5,7 @@
 // inside f16), so the attention kernels multiply f16 x f16 into f32: K and V
 // enter without rounding, the softmax weights keep 11 bits instead of bf16's 8,
 // and q (bf16) is scaled by a power of two per head row so that it fits f16
-// exactly except for elements more than 2^29 below the row's largest.  (Decode's
-// scores multiply the codes themselves, see attention_fp8.cu.)
+// exactly except for elements more than 2^29 below the row's largest.
 #pragma once
 
 #include <cuda_fp16.h>

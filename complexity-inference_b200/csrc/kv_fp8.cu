@@ -24,6 +24,10 @@
 // took 242 registers and left one CTA on an SM: 141 us for 8k rows.)  q rows are
 // rotated by further CTAs of the same launch.
 //
+// Bound: HBM by the bytes (q|k|v read, q and codes written), in fact latency: 8,000
+// rows of 32 + 16 heads of 128 take 52 us = 3.7 TB/s, the floor is 29; 256 decode
+// rows take 6.3 us, one 4.3 (an empty launch ~3).
+//
 // The rotation is a*c - b*s with every product rounded (no fused multiply-add)
 // and the QK-norm factor is formed in f64: next to a rounding border of e4m3 the
 // last bits of f32 decide, and these make the codes independent of the order of
@@ -63,7 +67,9 @@ struct KvFp8Args {
 
 constexpr int kWindow = 16;          // batch rows of a window CTA: the runs that start in them are its own
 constexpr int kAppendThreads = 256;
-constexpr int kAppendCtas = 3;      // resident per SM: 48 registers; 3 (79 registers) was 80 us for 8k rows, 5 is 61
+// Resident per SM: 80 registers, enough for the loads ahead of large steps.  (Before those,
+// 5 CTAs of 48 registers were faster, 61 us for 8k rows to 80; with them 3 take 52.)
+constexpr int kAppendCtas = 3;
 
 // 8 + 8 elements of a head: i0 .. i0+7 of the first half and their partners.
 __device__ __forceinline__ void unpack16(const uint4& lo, const uint4& hi, float (&x)[16]) {

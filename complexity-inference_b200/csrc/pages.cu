@@ -6,7 +6,8 @@
 // page one contiguous run; the 8-bit pool's block scales are a second set of
 // planes and move in the same launch.  Pure copy, bound by HBM: 2 * n * planes *
 // page bytes.  One CTA copies one page of one plane, four 16-byte loads a thread
-// in flight.  The pairs ride in the kernel's parameters, so a call needs no
+// in flight: 600 pages of 32 KB in 24 planes take 152 us = 6.2 TB/s (95 % of a plain
+// copy), 64 of 16 KB in 64 planes 24.4 us = 5.5 TB/s.  The pairs ride in the kernel's parameters, so a call needs no
 // device list, no copy of one and no synchronisation.
 #include <stdlib.h>
 
