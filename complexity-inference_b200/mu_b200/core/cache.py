@@ -281,21 +281,19 @@ class PagedKVCache:
             own = [p for p, _ in pairs if self.request_pos[p] < self.block_size]
             if len(own) > len(self.free_blocks):
                 return False
-            src, dst = [], []
-            for parent, child in pairs:
-                blocks, pos = self.request_blocks[parent], self.request_pos[parent]
-                shared = blocks if pos == self.block_size else blocks[:-1]
-                table = list(shared)
-                if pos < self.block_size:
-                    table.append(self.free_blocks.pop())
-                    if pos:
-                        src.append(blocks[-1])
-                        dst.append(table[-1])
-                for b in shared:
+            fresh = dict(zip((i for i, (p, _) in enumerate(pairs)
+                              if self.request_pos[p] < self.block_size), reversed(self.free_blocks)))
+            copies = [(self.request_blocks[pairs[i][0]][-1], b) for i, b in fresh.items()
+                      if self.request_pos[pairs[i][0]]]
+            self._copy_blocks([s for s, _ in copies], [d for _, d in copies])
+            for i, (parent, child) in enumerate(pairs):  # the device work is under way: book it
+                table = list(self.request_blocks[parent])
+                if i in fresh:
+                    table[-1] = self.free_blocks.pop()
+                for b in table[:-1] if i in fresh else table:
                     self.block_refs[b] = self.block_refs.get(b, 1) + 1
                 self.request_blocks[child] = table
-                self.request_pos[child] = pos
-            self._copy_blocks(src, dst)
+                self.request_pos[child] = self.request_pos[parent]
             return True
 
     def compact(self) -> int:

@@ -105,6 +105,25 @@ def test_fork_refused_changes_nothing(pairs):
     assert _same(want, _content(c, "a"))
 
 
+def test_failed_copy_changes_nothing():
+    c = _cache(FP8)
+    for r in "ab":
+        c.allocate(r)
+        _fill(c, r, 6, 1)
+    c.free("a")
+    state = (dict(c.request_blocks), dict(c.request_pos), list(c.free_blocks), dict(c.block_refs))
+
+    def fails(src, dst):
+        raise RuntimeError("launch")
+
+    c._copy_blocks = fails
+    with pytest.raises(RuntimeError):
+        c.fork("b", "c")
+    with pytest.raises(RuntimeError):
+        c.compact()
+    assert state == (c.request_blocks, c.request_pos, c.free_blocks, c.block_refs)
+
+
 @pytest.mark.parametrize("dtype", KINDS)
 def test_compact(dtype):
     c = _cache(dtype, blocks=24)
