@@ -17,7 +17,7 @@
 // probability, and O / l is the softmax average.  m only moves when a block exceeds it
 // by more than 8 (w <= 2^8), so O is rescaled on those blocks alone.
 //
-// Schedule.  Up to eight neighbouring KV heads are a group, a warp each, walking the same
+// Schedule.  Up to four or eight neighbouring KV heads are a group, a warp each, walking the same
 // blocks side by side (their tiles are neighbours in memory).  The blocks of all (sequence,
 // group) pairs, laid end to end, are cut into equal runs, one per warp group of a grid that
 // fills the GPU once; a warp's cp.async ring runs on across the pairs of its run.  A pair
@@ -26,12 +26,13 @@
 // tokens), or there are more than 2,048 of them, a warp takes whole pairs and nothing is
 // joined.
 //
-// Measured (32 query heads on 8, head_dim 128): 256 sequences of 200 to 1,500 tokens 90 us
-// (4.9 TB/s; floor 68), 32 of up to 32k 196 us (5.8 TB/s; floor 171; ~206 once the power cap
-// lowers the clock).  What bounds it now is the warps' chains of conversion, mma.sync and
-// exponentials, two warps per SM sub-partition: the same copies without them take 169 us as
-// 16 KB pieces.  Tried: such pieces by tensor copies from a loading warp 200 us, 2 KB tensor
-// copies per warp 221, four blocks ahead 200, 12 or 16 warps of fewer registers 201 to 216.
+// Measured (32 query heads on 8, head_dim 128): 256 sequences of 200 to 1,500 tokens 91 us
+// (4.9 TB/s; floor 68), 32 of up to 32k 202 us (5.6 TB/s; floor 171), also where the power
+// cap lowers the clock.  What bounds it now is the warps' chains of conversion, mma.sync and
+// exponentials, three warps per SM sub-partition: the same copies without them take 169 us as
+// 16 KB pieces.  Tried: such pieces by tensor copies from a loading warp 200 us (210 under
+// the cap, 97 for the short sequences), 2 KB tensor copies per warp 221, 16 warps of fewer
+// registers 213.
 //
 // Fragments: ldmatrix (plain for K, transposed for V) on 8-bit rows hands each lane four
 // neighbouring codes; the k (for V: m) index inside an MMA is a free permutation, chosen
@@ -51,9 +52,19 @@
 
 namespace muk {
 
-constexpr int kQdWarps = 8;        // warps per decode CTA, one CTA per SM
-constexpr int kQdAhead = 2;        // blocks on their way, per warp
-constexpr int kQdStages = 2 + kQdAhead;  // cp.async ring per warp: two more in work
+// Warps per decode CTA, one CTA per SM (registers: 168 or 255 a thread), blocks on their way
+// per warp, KV heads side by side at most.  Groups of up to 8 query heads: under the power
+// cap, where the chains of a warp take longer, 12 warps in groups of four heads with one block
+// ahead take 203 us for 32 sequences of up to 32k and 8 in a group with two ahead 217 (at full
+// clock 202 and 196); two ahead of 12 warps were 216, one ahead of 8 warps 222.  Larger groups
+// need the registers of 8.
+template <int NT>
+struct DecodeFp8Shape {
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kAhead = NT == 1 ? 1 : 2;
+  static constexpr int kHeads = NT == 1 ? 4 : 8;
+  static constexpr int kStages = 2 + kAhead;  // cp.async ring per warp: two more in work
+};
 // Blocks of a run, at least: a shorter one costs more in its pair's join than it saves
 // (and a pair's partial results stay within kQdMaxParts).
 constexpr int kQdMinRun = 12;
@@ -105,11 +116,11 @@ __device__ __forceinline__ int64_t decode_run(int64_t total, int runs, int min_r
   return r < min_run ? min_run : r;
 }
 
-template <int D>
+template <int D, int NT>
 struct DecodeFp8Smem {
   static constexpr int kTile = kKvBlock * D;            // bytes of one K (or V) block
   static constexpr int kStage = 2 * kTile + 16;         // K, V, two scales (+ pad)
-  static constexpr int kRing = kQdWarps * kQdStages * kStage;
+  static constexpr int kRing = DecodeFp8Shape<NT>::kWarps * DecodeFp8Shape<NT>::kStages * kStage;
 };
 
 // 2^x, one MUFU op (~2 ulp), far below what the f16 weight keeps.
@@ -125,13 +136,15 @@ struct DecodePlace {
 
 // NT: 8-head column groups (1: groups of up to 8 query heads, 2: up to 16).
 template <int D, int NT>
-__global__ void __launch_bounds__(kQdWarps * 32, 1)
+__global__ void __launch_bounds__(DecodeFp8Shape<NT>::kWarps * 32, 1)
     decode_fp8_kernel(const DecodeFp8Args a) {
   // programmatic dependent launch: let the next kernel launch once every CTA
   // of this one runs, and wait for the previous kernel before touching memory
   grid_dep_launch();
   grid_dep_wait();
-  using S = DecodeFp8Smem<D>;
+  using S = DecodeFp8Smem<D, NT>;
+  constexpr int kWarps = DecodeFp8Shape<NT>::kWarps, kAhead = DecodeFp8Shape<NT>::kAhead;
+  constexpr int kStages = DecodeFp8Shape<NT>::kStages;
   constexpr int kMT = D / 16;   // k steps of S, and m tiles of O
   extern __shared__ __align__(128) uint8_t smem[];
   int* prefix = reinterpret_cast<int*>(smem + S::kRing);  // [num_seqs + 1] blocks before a sequence
@@ -140,7 +153,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
   const int g = lane >> 2, tq = lane & 3;
   const int Hkv = a.num_kv_heads, G = a.num_q_heads / Hkv;
   // a run belongs to a group of warps, each with a head of its own
-  const int wid = (int)blockIdx.x * (kQdWarps / a.heads) + warp / a.heads, sub = warp % a.heads;
+  const int wid = (int)blockIdx.x * (kWarps / a.heads) + warp / a.heads, sub = warp % a.heads;
   const int NG = Hkv / a.heads;  // head groups of a sequence
 
   // rows of empty sequences are zero; too long ones are latched and left out
@@ -161,8 +174,8 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
   if (flat) {
     // prefix sums of the block counts, an equal share of the sequences per thread; the first
     // CTA leaves them for the join
-    __shared__ int s_sum[kQdWarps];
-    const int per = (a.num_seqs + kQdWarps * 32 - 1) / (kQdWarps * 32);
+    __shared__ int s_sum[kWarps];
+    const int per = (a.num_seqs + kWarps * 32 - 1) / (kWarps * 32);
     const int lo = min((int)threadIdx.x * per, a.num_seqs), hi = min(lo + per, a.num_seqs);
     int sum = 0;
     for (int b = lo; b < hi; ++b) sum += decode_blocks(a.seq_lens, b, a.max_blocks);
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
     __syncthreads();
     int before = upto - sum;
 #pragma unroll
-    for (int w = 0; w < kQdWarps; ++w) before += w < warp ? s_sum[w] : 0;
+    for (int w = 0; w < kWarps; ++w) before += w < warp ? s_sum[w] : 0;
     for (int b = lo; b < hi; ++b) {
       prefix[b] = before;
       before += decode_blocks(a.seq_lens, b, a.max_blocks);
@@ -219,7 +232,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
 
     // ---- loads: chunks of up to 32 blocks of one pair, an id per lane, the next
     // chunk's ids on their way
-    const uint32_t wbase = smem_u32(smem) + (uint32_t)(warp * kQdStages * S::kStage);
+    const uint32_t wbase = smem_u32(smem) + (uint32_t)(warp * kStages * S::kStage);
     DecodePlace nx = at;       // the next chunk's start
     int64_t nx_left = left;    // blocks from there to the run's end
     int cnt = 0, pos = 0, head = 0, ids = 0, nx_cnt = 0, nx_ids = 0;
@@ -235,6 +248,10 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
       if (to_issue > 0) {
         if (pos == cnt) {
           ids = nx_ids;
+          if (ids < 0 || ids >= a.num_blocks) {  // (lanes behind the chunk hold 0)
+            set_device_error(kDevBadIndex);
+            ids = 0;
+          }
           cnt = nx_cnt;
           pos = 0;
           head = nx.h * a.heads + sub;
@@ -252,11 +269,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
           }
           if (nx_left > 0) fetch();
         }
-        int id = __shfl_sync(0xffffffffu, ids, pos);
-        if (id < 0 || id >= a.num_blocks) {
-          if (lane == 0) set_device_error(kDevBadIndex);
-          id = 0;
-        }
+        const int id = __shfl_sync(0xffffffffu, ids, pos);
         const int64_t tile = (int64_t)id * Hkv + head;
         const uint8_t* ks = a.k_cache + tile * S::kTile + lane * 16;
         const uint8_t* vs = a.v_cache + tile * S::kTile + lane * 16;
@@ -272,12 +285,12 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
         if (lane < 2) cp_async_4(st + 2 * S::kTile + 4 * lane, (lane == 0 ? a.k_scale : a.v_scale) + tile);
         ++pos;
         --to_issue;
-        st_in = st_in + 1 == kQdStages ? 0 : st_in + 1;
+        st_in = st_in + 1 == kStages ? 0 : st_in + 1;
       }
       cp_async_commit();
     };
 #pragma unroll 1
-    for (int i = 0; i < kQdAhead; ++i) issue();
+    for (int i = 0; i < kAhead; ++i) issue();
 
     // ---- pair by pair
     int st_out = 0;
@@ -337,7 +350,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
         const bool two = i + 1 < n;  // else the second is absent: no row of it counts
         issue();
         if (two) issue();
-        cp_async_wait<kQdAhead>();
+        cp_async_wait<kAhead>();
         __syncwarp();
         uint32_t st[2];
         int rows[2];                 // tokens of the sequence from each block on
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int slot = st_out + p;
-          st[p] = wbase + (uint32_t)((slot >= kQdStages ? slot - kQdStages : slot) * S::kStage);
+          st[p] = wbase + (uint32_t)((slot >= kStages ? slot - kStages : slot) * S::kStage);
           rows[p] = ctx - (page0 + i + p) * kKvBlock;
           ks[p] = clamp_scale(ld_shared_f32(st[p] + 2 * S::kTile));
           const float vs = clamp_scale(ld_shared_f32(st[p] + 2 * S::kTile + 4));
@@ -359,7 +372,7 @@ __global__ void __launch_bounds__(kQdWarps * 32, 1)
         }
         const bool ragged = rows[0] < kKvBlock || rows[1] < kKvBlock;
         st_out += two ? 2 : 1;
-        if (st_out >= kQdStages) st_out -= kQdStages;
+        if (st_out >= kStages) st_out -= kStages;
 
         // S^T: rows = tokens
         float s[2][NT][4];
@@ -623,8 +636,10 @@ static int sm_count() {
 
 template <int D, int NT>
 static int launch_decode_fp8(DecodeFp8Args a, cudaStream_t stream) {
-  constexpr size_t most = DecodeFp8Smem<D>::kRing + (kQdFlatSeqs + 1) * sizeof(int);
-  const size_t smem = DecodeFp8Smem<D>::kRing + (a.max_parts > 0 ? (a.num_seqs + 1) * sizeof(int) : 0);
+  using Shape = DecodeFp8Shape<NT>;
+  constexpr size_t most = DecodeFp8Smem<D, NT>::kRing + (kQdFlatSeqs + 1) * sizeof(int);
+  static_assert(most <= 232448 - 64, "decode ring exceeds 227 KB of shared memory");
+  const size_t smem = DecodeFp8Smem<D, NT>::kRing + (a.max_parts > 0 ? (a.num_seqs + 1) * sizeof(int) : 0);
   static std::atomic<uint64_t> attr_done{0};
   const cudaError_t ae = smem_attr_once(decode_fp8_kernel<D, NT>, (int)most, attr_done);
   if (ae != cudaSuccess) {
@@ -632,16 +647,16 @@ static int launch_decode_fp8(DecodeFp8Args a, cudaStream_t stream) {
     return MUK_ERR_CUDA;
   }
   a.heads = 1;
-  while (a.heads < kQdWarps && a.num_kv_heads % (2 * a.heads) == 0) a.heads *= 2;
+  while (a.heads < Shape::kHeads && a.num_kv_heads % (2 * a.heads) == 0) a.heads *= 2;
   // a group of warps for each run of the shortest length, or pair, up to one resident grid
   const int64_t pairs = (int64_t)a.num_seqs * (a.num_kv_heads / a.heads);
   const int64_t work = a.max_parts > 0 ? pairs * ((a.max_blocks + a.min_run - 1) / a.min_run) : pairs;
-  const int per = kQdWarps / a.heads;
+  const int per = Shape::kWarps / a.heads;
   int64_t ctas = (work + per - 1) / per;
   const int64_t fill = sm_count();
   if (ctas > fill) ctas = fill;
   a.runs = (int)ctas * per;
-  launch_pdl(decode_fp8_kernel<D, NT>, dim3((unsigned)ctas), dim3(kQdWarps * 32), smem, stream, a);
+  launch_pdl(decode_fp8_kernel<D, NT>, dim3((unsigned)ctas), dim3(Shape::kWarps * 32), smem, stream, a);
   const int rc = check_launch("muk_paged_decode_attn_fp8");
   if (rc != MUK_OK || a.max_parts == 0) return rc;
   const int64_t items = (int64_t)a.num_seqs * a.num_kv_heads;
