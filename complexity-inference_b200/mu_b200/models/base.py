@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import os
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -239,6 +239,11 @@ class MuModelBase:
         self.kv_quantized = cache.quantized
         if cache.quantized and self.ws is not None:
             self.ws.add_fp8(self.config, self.device)
+
+    @staticmethod
+    def cache_key(cache) -> Tuple[int, int]:
+        """Where a cache's blocks and scales lie (0: no scales)."""
+        return (cache.block_pool.data_ptr(), cache.scales.data_ptr() if cache.quantized else 0)
 
     # ---- shared pieces of the step ---------------------------------------------
     def row_parallel(self, A: torch.Tensor, W: torch.Tensor, T: int, N: int) -> torch.Tensor:

@@ -162,7 +162,7 @@ class DeepForCausalLM(MuModelBase):
     def _native(self, cache) -> "_lib.MukDeepModel":
         """The executor's model struct (rebuilt when a buffer moves)."""
         ws, cfg, cl = self.ws, self.config, self.clamp
-        key = (id(ws), cache.block_pool.data_ptr(), cache.quantized, self.rope_cos.data_ptr(), id(self.comm),
+        key = (id(ws), self.cache_key(cache), self.rope_cos.data_ptr(), id(self.comm),
                self.fused_rope(), self._tp_fused, self.vocab_slice(), self.expert_lo,
                self.ep_combine)
         if key == self._native_key:
@@ -214,7 +214,7 @@ class DeepForCausalLM(MuModelBase):
             m.logits = ws.logits.data_ptr() + 4 * c0
         attn_ws = ws.attn_ws_fp8 if cache.quantized else ws.attn_ws
         m.attn_ws, m.attn_ws_bytes = attn_ws.data_ptr(), attn_ws.numel() * 4
-        m.kv_scales = cache.scales.data_ptr() if cache.quantized else 0
+        m.kv_scales = self.cache_key(cache)[1]
         m.fused_rope = int(self.fused_rope())
         m.tp_world, m.tp_rank = 1, 0
         m.tp_fused = FUSED_TP_MAX_ROWS if self._tp_fused else 0

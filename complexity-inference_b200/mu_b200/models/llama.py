@@ -135,7 +135,7 @@ class LlamaForCausalLM(MuModelBase):
     def _native(self, cache) -> "_lib.MukLlamaModel":
         """The executor's model struct (rebuilt when a buffer moves)."""
         ws, cfg = self.ws, self.config
-        key = (id(ws), cache.block_pool.data_ptr(), cache.quantized, self.rope_cos.data_ptr(), id(self.comm),
+        key = (id(ws), self.cache_key(cache), self.rope_cos.data_ptr(), id(self.comm),
                self.fused_rope(), self._tp_fused, self.fused_norm(), self.fused_norm_min_rows,
                self.tp_norm(), self.vocab_slice())
         if key == self._native_key:
@@ -172,7 +172,7 @@ class LlamaForCausalLM(MuModelBase):
             m.logits = ws.logits.data_ptr() + 4 * c0
         attn_ws = ws.attn_ws_fp8 if cache.quantized else ws.attn_ws
         m.attn_ws, m.attn_ws_bytes = attn_ws.data_ptr(), attn_ws.numel() * 4
-        m.kv_scales = cache.scales.data_ptr() if cache.quantized else 0
+        m.kv_scales = self.cache_key(cache)[1]
         m.fused_rope = int(self.fused_rope())
         m.tp_fused = FUSED_TP_MAX_ROWS if self._tp_fused else 0
         m.fused_norm = max(1, self.fused_norm_min_rows) if self.fused_norm() else 0

@@ -781,3 +781,34 @@ def test_captured_steps_and_side_streams(cuda):
         assert torch.equal(s["vc"].view(torch.uint8), t["vc"].view(torch.uint8))
         assert bool((t["out"][3] == 0).all())
     assert _err() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d,n", [(16, 8, 128, 40), (8, 8, 64, 20)])
+def test_blocks_behind_32_bit_offsets(cuda, hq, hkv, d, n):
+    """The last blocks of a cache of more than 2^32 bytes give the bits that the same blocks
+    of a small cache give: append, decode, prefill, copies."""
+    big = (1 << 32) // (hkv * BS * d) + 8
+    per = (n + BS - 1) // BS
+    qkv = torch.randn(n, (hq + 2 * hkv) * d, device="cuda", generator=_gen(71)).bfloat16()
+    cos, sin = _rope_tab(64, d)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    results = []
+    for nb in (big, 8):
+        kc, vc = (torch.zeros(nb, hkv, BS, d, dtype=torch.uint8, device="cuda").view(FP8) for _ in range(2))
+        ks, vs = (torch.ones(nb, hkv, device="cuda") for _ in range(2))
+        bt = torch.arange(nb - 1, nb - 1 - per, -1, dtype=torch.int32, device="cuda")[None]
+        slots = bt[0].long()[pos.long() // BS] * BS + pos.long() % BS
+        q = torch.empty(n, hq * d, dtype=torch.bfloat16, device="cuda")
+        _k().rope_kv_append_fp8(qkv, pos, slots.int(), cos, sin, hq, hkv, d, kc, vc, ks, vs, q_out=q)
+        sl = torch.tensor([n], dtype=torch.int32, device="cuda")
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        dec, pre = torch.empty_like(q[:1]), torch.empty_like(q)
+        _k().decode_attn_fp8(q[n - 1:], dec, kc, vc, ks, vs, bt, sl, hq, hkv, d, per * BS)
+        _k().prefill_attn_fp8(q, pre, kc, vc, ks, vs, bt, sl, cu, n, hq, hkv, d)
+        _k().copy_pages(kc, [nb - 1], [0], scales=ks)
+        assert _err() == 0
+        results.append((dec, pre, kc.view(torch.uint8)[bt[0].long()], ks[bt[0].long()],
+                        vc.view(torch.uint8)[bt[0].long()], kc.view(torch.uint8)[0], ks[0]))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert bool(results[0][2].any()) and torch.equal(results[0][2][0], results[0][5])

@@ -214,6 +214,22 @@ def test_bf16_and_8_bit_workers_share_a_model(cuda):
     assert not torch.equal(got["bf16"][0], got["fp8"][0])
 
 
+@pytest.mark.parametrize("name", ["llama_tiny", "deep_tiny"])
+def test_native_step_follows_moved_scales(cuda, name):
+    """Scales at another address beside a pool at the same one (a cache made anew)."""
+    w, d, prompts, _ = _worker(name, cuda)
+    for r in range(2):
+        assert w.allocate_request(f"r{r}")
+    reqs = [(f"r{r}", prompts[0]) for r in range(2)]
+    _logits(w, _requests(reqs[:1], True))
+    old = w.cache.scales
+    w.cache.scales = old.clone()
+    old.fill_(float("nan"))
+    _logits(w, _requests(reqs[1:], True))
+    assert bool(old.isnan().all())
+    assert bool(torch.isfinite(_logits(w, _requests([("r0", [3]), ("r1", [3])], False))).all())
+
+
 def test_shapes_that_are_not_built_are_refused(cuda):
     from mu_b200.core.cache import PagedKVCache
 
