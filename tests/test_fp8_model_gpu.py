@@ -14,13 +14,13 @@ from test_fp8_cache_gpu import _attend, _near
 pytestmark = pytest.mark.gpu
 
 
-def _worker(name, cuda, dtype="float8_e4m3", graphs=False, native=True, max_batch=8):
+def _worker(name, cuda, dtype="float8_e4m3", graphs=False, native=True, max_batch=8, blocks=256):
     from mu_b200.core.config import CacheConfig, EngineConfig, MuConfig, SchedulerConfig
     from mu_b200.serving.worker import MuWorker
 
     shape, cfg, sd, d, prompts = load_tiny(name)
     ec = EngineConfig(model=cfg, mu=MuConfig(enabled=True),
-                      cache=CacheConfig(max_seq_len=256, max_num_blocks=256, max_num_seqs=16,
+                      cache=CacheConfig(max_seq_len=256, max_num_blocks=blocks, max_num_seqs=16,
                                         dtype=dtype),
                       scheduler=SchedulerConfig(max_batch_size=max_batch,
                                                 max_num_batched_tokens=2048))
@@ -172,15 +172,17 @@ def test_forked_request(cuda, name, dtype):
     assert len(w.cache.free_blocks) == w.cache.max_num_blocks
 
 
-def test_engine_generates_the_decisive_tokens(cuda):
+@pytest.mark.parametrize("blocks", [256, 30])
+def test_engine_generates_the_decisive_tokens(cuda, blocks):
     """Greedy generation with the 8-bit cache, continuous batching and CUDA graphs: the
     fixture's residual stream stays close to the token's embedding (top-2 gap above 1
     at every step), and attention, whose rows alone change with the cache's rounding,
-    moves its logits far less than that."""
+    moves its logits far less than that.  A pool of 30 blocks holds about half of the
+    requests: others are preempted and prefilled again into blocks that held theirs."""
     from mu_b200.core.config import SamplingParams
     from mu_b200.serving.engine import StepEngine
 
-    w, d, prompts, ec = _worker("llama_decisive", cuda, graphs=True, max_batch=7)
+    w, d, prompts, ec = _worker("llama_decisive", cuda, graphs=True, max_batch=7, blocks=blocks)
     toks = d["tokens"]
     R, n = toks.shape
     eng = StepEngine(w, ec)
