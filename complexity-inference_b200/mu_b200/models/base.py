@@ -241,9 +241,11 @@ class MuModelBase:
             self.ws.add_fp8(self.config, self.device)
 
     @staticmethod
-    def cache_key(cache) -> Tuple[int, int]:
-        """Where a cache's blocks and scales lie (0: no scales)."""
-        return (cache.block_pool.data_ptr(), cache.scales.data_ptr() if cache.quantized else 0)
+    def cache_key(cache) -> Tuple[int, int, int, int]:
+        """Where a cache's blocks and scales lie (0: no scales) and what the planes of its
+        layers are counted in: another cache may get the same addresses."""
+        return (cache.block_pool.data_ptr(), cache.scales.data_ptr() if cache.quantized else 0,
+                cache.max_num_blocks, cache.block_size)
 
     # ---- shared pieces of the step ---------------------------------------------
     def row_parallel(self, A: torch.Tensor, W: torch.Tensor, T: int, N: int) -> torch.Tensor:
