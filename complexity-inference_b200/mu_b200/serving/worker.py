@@ -326,7 +326,8 @@ class MuWorker:
             K.fill_decode_inputs(batch.input_ids, batch.decode_src, sampled, st.patch)
         if not st.graph:
             return self.model.forward_step(batch, self.cache), batch
-        key = (self.packer.generation, id(self.model.ws))
+        # a graph holds the addresses, kernels and sizes of the cache it was captured with
+        key = (self.packer.generation, id(self.model.ws), self.model.cache_key(self.cache))
         if self._graph_key != key:
             self._graphs.clear()
             self._graph_key = key

@@ -2,6 +2,9 @@
 cache, on the CPU: addresses alone do not tell two caches apart, since a smaller pool may
 be carved from the start of a freed one."""
 
+import contextlib
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -35,3 +38,68 @@ def test_key_tells_pools_at_one_address_apart(dtype):
         b = _at(other, a)
         assert b.block_pool.data_ptr() == a.block_pool.data_ptr()
         assert MuModelBase.cache_key(b) != key
+
+
+class _Graph:
+    """A captured graph: replays what the model did under the capture."""
+
+    def __init__(self):
+        self.steps, self.replays = [], 0
+
+    def replay(self):
+        self.replays += 1
+
+
+@pytest.fixture
+def graphs(monkeypatch):
+    """torch.cuda's graph calls without a device."""
+    stream = SimpleNamespace(wait_stream=lambda s: None)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda: stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", _Graph)
+    monkeypatch.setattr(torch.cuda, "graph", lambda g: contextlib.nullcontext())
+
+
+def _graph_worker(cache):
+    from mu_b200.core.config import EngineConfig
+    from mu_b200.serving.step import StepPacker
+    from mu_b200.serving.worker import MuWorker
+
+    w = MuWorker(EngineConfig(), "cpu")
+    w.cache, w.packer = cache, StepPacker("cpu", 16, 4, 4)
+    seen = []
+    w.model = SimpleNamespace(ws=SimpleNamespace(logits=torch.zeros(4, 8)), tp_group=None,
+                              ensure_workspace=lambda *a: False, cache_key=MuModelBase.cache_key,
+                              forward_step=lambda batch, c: seen.append(c))
+    return w, seen
+
+
+def _decode(w, rid):
+    seqs, errors = w.prepare([(rid, [1])], 1)
+    assert not errors
+    w.run_step(seqs, 1)
+
+
+def test_graphs_follow_the_cache(graphs):
+    """A decode step after the cache was replaced, or its blocks or scales moved, is
+    captured anew; steps over an unchanged cache are replayed."""
+    big = _cache(12, FP8)
+    w, seen = _graph_worker(big)
+
+    def replayed():
+        n = len(seen)
+        _decode(w, "a")
+        assert all(c is w.cache for c in seen[n:])
+        return len(seen) == n
+
+    for cache in (big, _cache(12, torch.bfloat16), _at(_cache(8, FP8), big)):
+        w.cache = cache
+        assert w.allocate_request("a")
+        assert not replayed() and replayed() and replayed()
+    w.cache.scales = w.cache.scales.clone()
+    assert not replayed() and replayed()
+    w.cache.block_pool = w.cache.block_pool.clone()
+    assert not replayed() and replayed()
+    w.cache = big  # not what an older capture held
+    assert not replayed() and replayed()

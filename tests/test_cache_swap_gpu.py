@@ -56,3 +56,40 @@ def test_smaller_cache_in_the_memory_of_another(cuda, name, dtype):
     got = _run(w, prompts, "b")
     ref, _, _, _ = _worker(name, cuda, dtype=dtype, blocks=64)
     assert _same(got, _run(ref, prompts, "b")) and _same(_pool(w.cache), _pool(ref.cache))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("name", ["llama_tiny", "deep_tiny"])
+def test_graphs_of_caches_in_turn(cuda, name, native):
+    """Caches of both kinds and of two sizes in turn under one worker with graphs, each
+    decode from a bucket that was captured before the swap."""
+    caches = [("bfloat16", 256), ("float8_e4m3", 256), ("float8_e4m3", 64), ("bfloat16", 64)]
+    w, _, prompts, _ = _worker(name, cuda, dtype=caches[0][0], graphs=True, native=native)
+    live = [w.cache] + [_cache(w, n, dtype) for dtype, n in caches[1:]]
+    got = [[] for _ in caches]
+    for turn in range(2):
+        for i, c in enumerate(live):
+            w.cache = c
+            got[i] += _run(w, prompts, f"r{turn}")
+    for i, (dtype, n) in enumerate(caches):
+        ref, _, _, _ = _worker(name, cuda, dtype=dtype, graphs=True, native=native, blocks=n)
+        want = _run(ref, prompts, "r0") + _run(ref, prompts, "r1")
+        assert ref.get_stats()["cuda_graphs"] and _same(got[i], want), (dtype, n)
+        assert _same(_pool(live[i]), _pool(ref.cache)), (dtype, n)
+
+
+@pytest.mark.parametrize("name", ["llama_tiny", "deep_tiny"])
+def test_graphs_follow_moved_memory(cuda, name):
+    """Scales, then blocks, at other addresses between two decodes of a captured bucket."""
+    w, _, prompts, _ = _worker(name, cuda, graphs=True)
+    ref, _, _, _ = _worker(name, cuda, graphs=True)
+    assert _same(_run(w, prompts, "a"), _run(ref, prompts, "a"))
+    for part in ("scales", "block_pool"):
+        old = getattr(w.cache, part)
+        setattr(w.cache, part, old.clone())
+        old.view(torch.uint8).fill_(0x7F)
+        kept = old.view(torch.uint8).clone()
+        for tok in (9, 10):
+            step = _requests([("a", [tok])], False)
+            assert torch.equal(_logits(w, step), _logits(ref, step))
+        assert torch.equal(old.view(torch.uint8), kept) and _same(_pool(w.cache), _pool(ref.cache))
