@@ -14,6 +14,7 @@ table built exactly as RotaryEmbeddingCompat builds it (layers.py:286-299).
 
 from __future__ import annotations
 
+import itertools
 import os
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Tuple
@@ -86,7 +87,10 @@ class Workspace:
     """Activation buffers sized for ``max_tokens`` tokens / ``max_seqs`` sequences.
 
     Buffer addresses stay fixed for the life of the workspace, which is what
-    lets a decode step be captured in a CUDA graph and replayed."""
+    lets a decode step be captured in a CUDA graph and replayed.  ``serial`` names it
+    among all workspaces (an ``id`` may come back after a workspace was dropped)."""
+
+    _serials = itertools.count(1)
 
     def __init__(self, model: "MuModelBase", max_tokens: int, max_seqs: int, max_seq_len: int):
         cfg = model.config
@@ -95,6 +99,7 @@ class Workspace:
         Hq, Hkv = cfg.num_attention_heads, cfg.num_key_value_heads
         T = max_tokens
         self.max_tokens, self.max_seqs, self.max_seq_len = T, max_seqs, max_seq_len
+        self.serial = next(Workspace._serials)
         bf, f32 = torch.bfloat16, torch.float32
         self.resid = torch.empty(T, H, device=dev, dtype=f32)
         # [x | mu_prev] for Deep; under peer-memory TP the model may keep x in

@@ -162,7 +162,7 @@ class DeepForCausalLM(MuModelBase):
     def _native(self, cache) -> "_lib.MukDeepModel":
         """The executor's model struct (rebuilt when a buffer moves)."""
         ws, cfg, cl = self.ws, self.config, self.clamp
-        key = (id(ws), self.cache_key(cache), self.rope_cos.data_ptr(), id(self.comm),
+        key = (ws.serial, self.cache_key(cache), self.rope_cos.data_ptr(), id(self.comm),
                self.fused_rope(), self._tp_fused, self.vocab_slice(), self.expert_lo,
                self.ep_combine)
         if key == self._native_key:

@@ -135,7 +135,7 @@ class LlamaForCausalLM(MuModelBase):
     def _native(self, cache) -> "_lib.MukLlamaModel":
         """The executor's model struct (rebuilt when a buffer moves)."""
         ws, cfg = self.ws, self.config
-        key = (id(ws), self.cache_key(cache), self.rope_cos.data_ptr(), id(self.comm),
+        key = (ws.serial, self.cache_key(cache), self.rope_cos.data_ptr(), id(self.comm),
                self.fused_rope(), self._tp_fused, self.fused_norm(), self.fused_norm_min_rows,
                self.tp_norm(), self.vocab_slice())
         if key == self._native_key:

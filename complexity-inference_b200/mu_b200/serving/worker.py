@@ -327,7 +327,7 @@ class MuWorker:
         if not st.graph:
             return self.model.forward_step(batch, self.cache), batch
         # a graph holds the addresses, kernels and sizes of the cache it was captured with
-        key = (self.packer.generation, id(self.model.ws), self.model.cache_key(self.cache))
+        key = (self.packer.generation, self.model.ws.serial, self.model.cache_key(self.cache))
         if self._graph_key != key:
             self._graphs.clear()
             self._graph_key = key

@@ -69,7 +69,7 @@ def _graph_worker(cache):
     w = MuWorker(EngineConfig(), "cpu")
     w.cache, w.packer = cache, StepPacker("cpu", 16, 4, 4)
     seen = []
-    w.model = SimpleNamespace(ws=SimpleNamespace(logits=torch.zeros(4, 8)), tp_group=None,
+    w.model = SimpleNamespace(ws=SimpleNamespace(serial=1, logits=torch.zeros(4, 8)), tp_group=None,
                               ensure_workspace=lambda *a: False, cache_key=MuModelBase.cache_key,
                               forward_step=lambda batch, c: seen.append(c))
     return w, seen
@@ -103,3 +103,26 @@ def test_graphs_follow_the_cache(graphs):
     assert not replayed() and replayed()
     w.cache = big  # not what an older capture held
     assert not replayed() and replayed()
+
+
+@pytest.mark.parametrize("name", ["llama_tiny", "deep_tiny"])
+def test_native_step_follows_the_workspace(name):
+    """Two growths between two steps: the second workspace may be the Python object of
+    the one before the first (the interpreter reuses its place)."""
+    from golden_models import load_tiny
+    from mu_b200 import _lib
+    from mu_b200.models.loader import build_model
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libmuk.so not built (run complexity-inference_b200/build.py)")
+    shape, cfg, sd, _, _ = load_tiny(name)
+    m = build_model(shape.arch, cfg, sd, MuConfig(enabled=True), "cpu")
+    c = PagedKVCache(cfg.num_hidden_layers, cfg.num_key_value_heads, cfg.head_dim, 16, 4,
+                     torch.bfloat16, "cpu")
+    m.use_cache(c)
+    for n in range(64, 128, 2):
+        m.ensure_workspace(n, 2, 64)
+        assert m._native(c).qkv == m.ws.qkv.data_ptr()
+        for more in (1, 2):
+            m.ensure_workspace(n + more, 2, 64)
+        assert m._native(c).qkv == m.ws.qkv.data_ptr()
