@@ -701,17 +701,18 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
         get_ml(s, m, x);
         M = fmaxf(M, m);
       }
-      // a row without a bound has seen no key (l 0), or NaN alone
-      auto factor = [&](float m, float x) {
-        return m == -INFINITY ? (x != 0.f ? 1.f : 0.f) : x_exp2(m - M);
-      };
-      const float own = factor(m_used, l);
-      float L = own != 0.f ? own * l : 0.f;
+      // A row without a bound has seen no key (l 0: its O is not read), or NaN alone.  Every
+      // other share counts, however small its factor: the bound ignores NaN, which l and O
+      // hold, and 0 * NaN is NaN.
+      auto live = [&](float m, float x) { return m != -INFINITY || x != 0.f; };
+      auto factor = [&](float m) { return m == -INFINITY ? 1.f : x_exp2(m - M); };
+      const bool has = live(m_used, l);
+      const float own = factor(m_used);
+      float L = has ? own * l : 0.f;
       for (int s = 0; s < splits - 1; ++s) {
         float m, x;
         get_ml(s, m, x);
-        const float f = factor(m, x);
-        if (f != 0.f) L = fmaf(f, x, L);
+        if (live(m, x)) L = fmaf(factor(m), x, L);
       }
       const float inv = 1.f / L;
 #pragma unroll 1
@@ -720,12 +721,12 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
         tmem_ld_wait();
         float o[32];
 #pragma unroll
-        for (int u = 0; u < 32; ++u) o[u] = own != 0.f ? own * __uint_as_float(rr[u]) : 0.f;
+        for (int u = 0; u < 32; ++u) o[u] = has ? own * __uint_as_float(rr[u]) : 0.f;
         for (int s = 0; s < splits - 1; ++s) {
           float m, x;
           get_ml(s, m, x);
-          const float f = factor(m, x);
-          if (f != 0.f) {
+          const float f = factor(m);
+          if (live(m, x)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 v = ld_shared_f4(box + (s * rows + my) * (kXD * 4) + (uint32_t)(((i * 8 + j) ^ lane) << 4));

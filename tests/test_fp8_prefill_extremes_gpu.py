@@ -1,0 +1,45 @@
+"""The 8-bit cache's prefill attention at the ends of its range: blocks that read as NaN
+beside keys of far larger scores, infinite queries, queries too small for f32 products,
+scales at both ends of [2^-60, 2^60].  Tolerances are those of test_fp8_cache_gpu."""
+
+import math
+
+import pytest
+import torch
+
+from test_fp8_cache_gpu import BS, FP8, _attend, _err, _gen, _k, _near, _quantised, _tables
+
+pytestmark = pytest.mark.gpu
+
+
+def _prefill(q, bt, lens, qn, kc, ks, vc, vs, hq, hkv, d):
+    cu = [0]
+    for n in qn:
+        cu.append(cu[-1] + n)
+    out = torch.full_like(q, 7.0)
+    _k().prefill_attn_fp8(q, out, kc, vc, ks, vs, bt, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                          torch.tensor(cu, dtype=torch.int32, device="cuda"), max(qn), hq, hkv, d)
+    assert _err() == 0
+    return out
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad,loud", [(0, 5), (3, 5), (7, 0), (5, 5)])
+def test_nan_block_below_far_larger_scores(cuda, bad, loud, which):
+    """The key tiles of 40 rows behind 9,000 tokens are shared out in eighths; a block of
+    eighth `bad` reads as NaN, the scores of eighth `loud` are hundreds of powers of two
+    above all others.  A row that sees the block is NaN all the same (0 * NaN)."""
+    hq, hkv, d, past, n = 4, 1, 128, 9000, 40
+    ctx = past + n
+    bt, nb = _tables([ctx], 3)
+    kc, ks = _quantised(nb, hkv, d, 71)
+    vc, vs = _quantised(nb, hkv, d, 72)
+    per = -(-(-(-ctx // 64)) // 8) * 4               # blocks of an eighth
+    high = bt[0, loud * per:min((loud + 1) * per, bt.shape[1])].long()
+    ks[high] *= 2.0 ** 9
+    q = torch.randn(n, hq * d, device="cuda", generator=_gen(73)).bfloat16()
+    want, bound = _attend(q.view(n, hq, d), kc, ks, vc, vs, bt[0], ctx,
+                          past + torch.arange(n, device="cuda"), d ** -0.5, hkv)
+    _near(_prefill(q, bt, [ctx], [n], kc, ks, vc, vs, hq, hkv, d), want, bound, "without NaN")
+    (ks if which == "k" else vs)[int(bt[0, bad * per + 5])] = float("nan")
+    assert bool(_prefill(q, bt, [ctx], [n], kc, ks, vc, vs, hq, hkv, d).isnan().all())
