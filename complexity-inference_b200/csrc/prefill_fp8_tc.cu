@@ -46,6 +46,7 @@
 //
 // Every wait is bounded (common.cuh); on time-out the kernel records the error
 // word, every role leaves its loop, TMEM is freed and the CTA returns.
+#include <float.h>
 #include <math.h>
 
 #include "abi_util.h"
@@ -594,7 +595,13 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
           const float4 k = cs[j];
           // a block that this row does not see must not reach it even as NaN
           const bool hidden = diagonal && k0 + 16 * j > limit;
-          const float kc = hidden ? 1.f : k.x * c, off = hidden ? 0.f : k.y - mu;
+          // A block of zeros has the smallest scale, and a row of tiny queries brings the
+          // product to 0: held to the smallest normal, at which every score is 0 all the
+          // same (|x| < 2^31), unseen keys stay -inf (a NaN scale stays NaN).
+          float kc = k.x * c;
+          kc = kc < FLT_MIN ? FLT_MIN : kc;
+          kc = hidden ? 1.f : kc;
+          const float off = hidden ? 0.f : k.y - mu;
           float sa = 0.f, sb2 = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {

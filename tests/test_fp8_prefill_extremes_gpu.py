@@ -43,3 +43,23 @@ def test_nan_block_below_far_larger_scores(cuda, bad, loud, which):
     _near(_prefill(q, bt, [ctx], [n], kc, ks, vc, vs, hq, hkv, d), want, bound, "without NaN")
     (ks if which == "k" else vs)[int(bt[0, bad * per + 5])] = float("nan")
     assert bool(_prefill(q, bt, [ctx], [n], kc, ks, vc, vs, hq, hkv, d).isnan().all())
+
+
+@pytest.mark.parametrize("past,n", [(0, 100), (9000, 40), (61, 3)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 128), (16, 8, 128), (4, 2, 64)])
+def test_tiny_query_over_zero_keys(cuda, hq, hkv, d, past, n):
+    """Keys of zeros (codes 0, the smallest scale, as the append writes them) on the
+    diagonal and queries of about 2^-90: scores are zero, not 0 * inf, and a row is the
+    average of the values that it sees."""
+    ctx = past + n
+    bt, nb = _tables([ctx], 7)
+    kc, ks = _quantised(nb, hkv, d, 91)
+    vc, vs = _quantised(nb, hkv, d, 92, spread=2.0)
+    zero = bt[0, past // BS:].long()
+    kc.view(torch.uint8)[zero] = 0
+    ks[zero] = 2.0 ** -60
+    q = (2.0 ** -90 * torch.randn(n, hq * d, device="cuda", generator=_gen(93))).bfloat16()
+    out = _prefill(q, bt, [ctx], [n], kc, ks, vc, vs, hq, hkv, d)
+    want, bound = _attend(q.view(n, hq, d), kc, ks, vc, vs, bt[0], ctx,
+                          past + torch.arange(n, device="cuda"), d ** -0.5, hkv)
+    _near(out, want, bound, f"{past} + {n}")
