@@ -63,3 +63,23 @@ def test_tiny_query_over_zero_keys(cuda, hq, hkv, d, past, n):
     want, bound = _attend(q.view(n, hq, d), kc, ks, vc, vs, bt[0], ctx,
                           past + torch.arange(n, device="cuda"), d ** -0.5, hkv)
     _near(out, want, bound, f"{past} + {n}")
+
+
+@pytest.mark.parametrize("value", [0.0, 1.0])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 128), (8, 1, 128), (4, 2, 64)])
+def test_infinite_query(cuda, hq, hkv, d, value):
+    """An infinite query element against codes that are negative for every key but one of
+    each sequence: that key's score is inf * 0 = NaN or inf, the others' -inf, and the
+    softmax of such a row is NaN, at every place of the key in its block."""
+    lens = [64] * 16
+    bt, nb = _tables(lens, 5)
+    kc, ks = _quantised(nb, hkv, d, 81)
+    vc, vs = _quantised(nb, hkv, d, 82)
+    kc = kc.float()
+    kc[..., 0] = -1.0
+    for b in range(16):
+        kc[int(bt[b, b % 4]), :, b, 0] = value
+    q = torch.randn(16, hq, d, device="cuda", generator=_gen(83)).bfloat16()
+    q[:, :, 0] = math.inf
+    out = _prefill(q.flatten(1), bt, lens, [1] * 16, kc.to(FP8), ks, vc, vs, hq, hkv, d)
+    assert bool(out.isnan().all())
