@@ -157,11 +157,12 @@ __device__ __forceinline__ float x_exp2(float x) {
 // 2^x on the FMA pipe, for a part of the weights (MUFU takes 8 clocks a warp, and was
 // busy 1,024 of a tile's ~2,200): 2^n * p(f), n = round(x) from the bits of x + 1.5 * 2^23
 // (127 more, so that they are 2^n's), f = x - n in [-1/2, 1/2], p the degree-4 minimax
-// polynomial of 2^f (relative error 2^-18.5, fitted for this; f16 keeps 2^-11).  Below
-// 2^-126 it returns 2^-126.  NaN stays NaN: a maximum that keeps it, and a product by 2^n
-// (n added to the exponent would make a number of it).
+// polynomial of 2^f (relative error 2^-18.5, fitted for this; f16 keeps 2^-11).  From
+// -126.5 down n is -127, whose bits are 0.0: an unseen key weighs nothing, whatever 1 / vs
+// its block has.  NaN stays NaN: a maximum that keeps it, and a product by 2^n (n added to
+// the exponent would make a number of it).
 __device__ __forceinline__ float x_exp2_fma(float x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-127.f));
   const float z = x + 12583039.f;
   const float f = x - (z - 12583039.f);
   float p = fmaf(f, 0.0095701013f, 0.0559178628f);

@@ -83,3 +83,31 @@ def test_infinite_query(cuda, hq, hkv, d, value):
     q[:, :, 0] = math.inf
     out = _prefill(q.flatten(1), bt, lens, [1] * 16, kc.to(FP8), ks, vc, vs, hq, hkv, d)
     assert bool(out.isnan().all())
+
+
+@pytest.mark.parametrize("past,n", [(0, 100), (9000, 40)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 128), (16, 8, 128), (4, 2, 64)])
+def test_values_of_both_ends_of_the_scale_range(cuda, hq, hkv, d, past, n):
+    """Blocks of zero values (the smallest scale) whose keys score far below the others',
+    whose values have the largest: the unseen and the faint keys add nothing to the sum."""
+    ctx = past + n
+    bt, nb = _tables([ctx], 8)
+    kc, ks = _quantised(nb, hkv, d, 94)
+    vc, vs = _quantised(nb, hkv, d, 95)
+    kf = kc.float()
+    kf[..., 0] = 448.0                               # the score of every key: about +-448 * 8 * scale
+    odd = torch.zeros(nb, dtype=torch.bool, device="cuda")
+    odd[bt[0, 1::2].long()] = True
+    kf[odd] = 0.0
+    kf[odd, ..., 0] = -448.0
+    kc = kf.to(FP8)
+    ks[:] = 2.0 ** -3
+    vs[:] = 2.0 ** 60
+    vc.view(torch.uint8)[odd] = 0
+    vs[odd] = 2.0 ** -60
+    q = torch.randn(n, hq, d, device="cuda", generator=_gen(96)).bfloat16()
+    q[:, :, 0] = 64.0
+    out = _prefill(q.flatten(1), bt, [ctx], [n], kc, ks, vc, vs, hq, hkv, d)
+    want, bound = _attend(q, kc, ks, vc, vs, bt[0], ctx, past + torch.arange(n, device="cuda"),
+                          d ** -0.5, hkv)
+    _near(out, want, bound, f"{past} + {n}")
