@@ -30,6 +30,7 @@ front of the pool.  Neither has a counterpart in the reference.
 from __future__ import annotations
 
 import threading
+from collections import Counter
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -218,12 +219,15 @@ class PagedKVCache:
     def block_table(self, request_id: str) -> List[int]:
         return self.request_blocks.get(request_id, [])
 
-    def held_blocks(self, request_id: str) -> int:
-        """Blocks that ``free`` would give back (those no other request shares)."""
+    def held_blocks(self, *request_ids: str) -> int:
+        """Blocks that freeing all of these requests would give back (those that no
+        other request shares)."""
         with self._lock:
-            blocks = self.request_blocks.get(request_id, [])
-            return sum(1 for b in blocks if b not in self.block_refs) if self.block_refs \
-                else len(blocks)
+            tables = [self.request_blocks.get(r, []) for r in request_ids]
+            if not self.block_refs:
+                return sum(len(t) for t in tables)
+            n = Counter(b for t in tables for b in t)
+            return sum(1 for b, k in n.items() if k == self.block_refs.get(b, 1))
 
     def free(self, request_id: str) -> None:
         with self._lock:

@@ -234,13 +234,16 @@ class MuScheduler:
         return preempted
 
     def fit_blocks(self, out: SchedulerOutput, free: int, need_of: Callable[[Request, int], int],
-                   held_of: Callable[[Request], int]) -> List[Request]:
+                   held_of: Callable[[Request], int],
+                   freed_of: Optional[Callable[[List[Request]], int]] = None) -> List[Request]:
         """Shrink a scheduled step until its new KV blocks fit the ``free`` ones.
 
         ``need_of(req, n)``: blocks that appending ``n`` tokens to ``req``
         takes (a request not yet in the cache counts its first block);
-        ``held_of(req)``: blocks ``req`` holds now.  The reference never runs
-        out of KV memory (its cache grows by ``torch.cat``), so this is an
+        ``held_of(req)``: blocks ``req`` holds now; ``freed_of(reqs)``: blocks
+        that come back when all of ``reqs`` are preempted (default: what they
+        hold; less where others share them).  The reference never runs out of
+        KV memory (its cache grows by ``torch.cat``), so this is an
         addition, in the reference's own terms.  In order:
 
         1. requests admitted by this ``schedule`` go back to the front of the
@@ -251,10 +254,10 @@ class MuScheduler:
            generated tokens first).
 
         Preemption is by recompute: the engine frees the request's blocks and
-        it re-prefills prompt + generated tokens when readmitted.  Every
-        preemption frees blocks, so the loop cannot cycle; a request that
-        does not fit an otherwise empty pool is left for the cache's
-        all-or-nothing reserve to reject.  Returns the requests preempted
+        it re-prefills prompt + generated tokens when readmitted, for which
+        it waits while others hold blocks, so preemption cannot cycle; a
+        request that does not fit with no other request running is left for
+        the cache's all-or-nothing reserve to reject.  Returns the requests preempted
         here (also appended to ``out.preempted_requests``)."""
         need = {id(r): need_of(r, 1) for r in out.decode_requests}
         for r, (_, n) in zip(out.prefill_requests, out.prefill_chunks):
@@ -288,10 +291,11 @@ class MuScheduler:
         victims = [r for r in reversed(out.prefill_requests) if held_of(r) > 0]
         victims += sorted(out.decode_requests, key=lambda r: r.num_generated_tokens, reverse=True)
         preempted: List[Request] = []
+        room = free
         for req in victims:
-            if total <= free:
+            if total <= room:
                 break
-            free += held_of(req)
+            room = free + freed_of(preempted + [req]) if freed_of else room + held_of(req)
             if req in out.prefill_requests:
                 drop_prefill(req)
             else:

@@ -250,8 +250,9 @@ class StepEngine:
         # a decode takes at most one new block, a chunk of n tokens at most n // bs + 2
         worst = len(out.decode_requests) + sum(n // bs + 2 for _, n in out.prefill_chunks)
         if worst > free:
-            for req in self.scheduler.fit_blocks(out, free, need_of,
-                                                 lambda r: cache.held_blocks(r.request_id)):
+            for req in self.scheduler.fit_blocks(
+                    out, free, need_of, lambda r: len(cache.block_table(r.request_id)),
+                    lambda reqs: cache.held_blocks(*(r.request_id for r in reqs))):
                 self._release(req.request_id)
         prefills: List[Request] = []
         chunks: List[tuple] = []
