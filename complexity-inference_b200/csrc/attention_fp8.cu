@@ -961,6 +961,8 @@ extern "C" int muk_paged_decode_attn_fp8(const void* q, int64_t q_stride, void* 
                   out_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0 &&
                   MUK_ALIGNED16(k_cache) && MUK_ALIGNED16(v_cache),
               "muk_paged_decode_attn_fp8: strides/alignment");
+  MUK_REQUIRE(num_seqs <= 1 || out_stride >= (int64_t)num_q_heads * head_dim,
+              "muk_paged_decode_attn_fp8: rows of out overlap (stride %lld)", (long long)out_stride);
   MUK_REQUIRE(scale > 0.f && scale <= 3.4e38f, "muk_paged_decode_attn_fp8: scale must be positive");
   MUK_REQUIRE(num_blocks > 0 && max_seq_len > 0 &&
                   (int64_t)block_table_stride * kKvBlock >= max_seq_len,
@@ -1037,6 +1039,8 @@ extern "C" int muk_paged_prefill_attn_fp8(const void* q, int64_t q_stride, void*
   MUK_REQUIRE(q_stride % 8 == 0 && out_stride % 8 == 0 && MUK_ALIGNED16(q) && MUK_ALIGNED16(out) &&
                   MUK_ALIGNED16(k_cache) && MUK_ALIGNED16(v_cache),
               "muk_paged_prefill_attn_fp8: strides/alignment");
+  MUK_REQUIRE(num_rows <= 1 || out_stride >= (int64_t)num_q_heads * head_dim,
+              "muk_paged_prefill_attn_fp8: rows of out overlap (stride %lld)", (long long)out_stride);
   MUK_REQUIRE(scale > 0.f && scale <= 3.4e38f, "muk_paged_prefill_attn_fp8: scale must be positive");
   MUK_REQUIRE(num_blocks > 0 && max_seq_len > 0 &&
                   (int64_t)block_table_stride * kKvBlock >= max_seq_len,

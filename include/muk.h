@@ -224,7 +224,8 @@ size_t muk_decode_attn_fp8_workspace_size(int num_seqs, int num_q_heads, int hea
                                           int max_seq_len, int block_size);
 
 /* muk_paged_decode_attn over the 8-bit cache.  Sequences with seq_lens[b] <= 0
- * get zero rows; scale > 0.  Contexts beyond the launch's size and bad block ids
+ * get zero rows; scale > 0; the rows of out do not overlap (out_stride at least
+ * num_q_heads * head_dim).  Contexts beyond the launch's size and bad block ids
  * latch device error 5 as there. */
 int muk_paged_decode_attn_fp8(const void* q, int64_t q_stride, void* out, int64_t out_stride,
                               const void* k_cache, const void* v_cache, const float* k_scale,
@@ -235,7 +236,7 @@ int muk_paged_decode_attn_fp8(const void* q, int64_t q_stride, void* out, int64_
                               size_t workspace_bytes, void* stream);
 
 /* muk_paged_prefill_attn over the 8-bit cache; scale > 0, strides multiples of 8,
- * q and out 16-byte aligned.  num_rows: rows of q and out; max_seq_len: largest
+ * the rows of out not overlapping, q and out 16-byte aligned.  num_rows: rows of q and out; max_seq_len: largest
  * context, which a block-table row holds.  A sequence whose rows do not lie in
  * [0, num_rows), whose seq_lens is below its q length or above max_seq_len's
  * blocks, or with more than max_q_len rows latches device error 4 and is skipped. */
