@@ -246,26 +246,26 @@ __device__ __forceinline__ void append_single(const KvFp8Args& a, int64_t item) 
   if (c == 0) *sc = scale_value(n);
 }
 
-// Up to 16 rows t .. t + rows - 1, all of block blk, of the K and V heads of groups g0 ..
-// g1 - 1 (kHeads neighbouring heads, K first, are a group): a warp has kPer rows of a
-// head, its lanes 16 elements each.  Every warp of the CTA calls it (one barrier a
-// group); the next group's rows are loaded while this one's are worked on.
+// Up to 16 rows, all of block blk, of the K and V heads of groups g0 .. g1 - 1 (kHeads
+// neighbouring heads, K first, are a group): lane i < 16 holds batch row tr (-1: none) and
+// its slot; of rows naming one slot the last counts.  A warp has kPer rows of a head, its
+// lanes 16 elements each.  Every warp of the CTA calls it (one barrier a group); the next
+// group's rows are loaded while this one's are worked on.
 template <int D>
-__device__ __forceinline__ void append_rows(const KvFp8Args& a, int t, int rows, int blk, int slot,
-                                            int g0, int g1, uint32_t (*red)[kAppendThreads / 32]) {
+__device__ __forceinline__ void append_rows(const KvFp8Args& a, int tr, int slot, int blk, int g0,
+                                            int g1, uint32_t (*red)[kAppendThreads / 32]) {
   constexpr int kLanes = D / 16;           // lanes of a row
   constexpr int kPer = 32 / kLanes;        // rows of a warp
   constexpr int kWph = kKvBlock / kPer;    // warps of a head
   constexpr int kHeads = kAppendThreads / 32 / kWph;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wq = warp % kWph;
   const int c = lane % kLanes, i0 = c * 8, r = wq * kPer + lane / kLanes;
-  // lane i holds row i's place; of rows naming one slot the last one counts
   const int off = slot - blk * kKvBlock;
-  const uint32_t same = __match_any_sync(0xffffffffu, lane < rows ? off : 64 + lane);
-  const bool valid = lane < rows && (31 - __clz(same)) == lane;
-  int pos = lane < rows ? a.positions[t + lane] : 0;
+  const uint32_t same = __match_any_sync(0xffffffffu, tr >= 0 ? off : 64 + lane);
+  const bool valid = tr >= 0 && (31 - __clz(same)) == lane;
+  int pos = tr >= 0 ? a.positions[tr] : 0;
   const bool pos_ok = pos >= 0 && pos < a.max_pos;
-  if (lane < rows && !pos_ok) {
+  if (tr >= 0 && !pos_ok) {
     set_device_error(kDevBadIndex);
     pos = 0;
   }
@@ -275,13 +275,13 @@ __device__ __forceinline__ void append_rows(const KvFp8Args& a, int t, int rows,
   const uint32_t ov = __reduce_or_sync(0xffffffffu, valid ? 1u << off : 0u);
   const int o = __shfl_sync(0xffffffffu, off, r), p = __shfl_sync(0xffffffffu, pos, r);
   const Rope8 rope = load_rope<D>(a, p, i0);
-  const __nv_bfloat16* row = a.qkv + (int64_t)(t + (r < rows ? r : 0)) * a.qkv_stride +
-                             (int64_t)a.num_q_heads * D + i0;
+  const int t = __shfl_sync(0xffffffffu, tr, r);
+  const __nv_bfloat16* row = a.qkv + (int64_t)max(t, 0) * a.qkv_stride + (int64_t)a.num_q_heads * D + i0;
   uint4 lo, hi;
   auto load = [&](int g) {
     const int j = g * kHeads + warp / kWph;
     lo = hi = make_uint4(0u, 0u, 0u, 0u);
-    if (j < 2 * a.num_kv_heads && r < rows) {
+    if (j < 2 * a.num_kv_heads && t >= 0) {
       lo = *reinterpret_cast<const uint4*>(row + (int64_t)j * D);
       hi = *reinterpret_cast<const uint4*>(row + (int64_t)j * D + D / 2);
     }
@@ -341,12 +341,12 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_kv_append_fp
     prev = prev < 0 ? -1 : prev / kKvBlock;
     // uniform over the CTA: every warp walks the same rows
     for (int t = t0; t < t1;) {
-      // lanes 0-15 look at the next rows; n of them are in row t's block
-      const int slot = lane < kKvBlock && t + lane < T ? a.slots[t + lane] : -1;
+      // the lanes look at the next rows: n of them are in row t's block
+      const int slot = t + lane < T ? a.slots[t + lane] : -1;
       const int blk_l = slot < 0 ? -1 : slot / kKvBlock;
       const int blk = __shfl_sync(0xffffffffu, blk_l, 0);
-      const uint32_t in = __ballot_sync(0xffffffffu, lane < kKvBlock && blk_l == blk);
-      const int n = in == 0xffffu ? kKvBlock : __ffs(~in) - 1;
+      const uint32_t in = __ballot_sync(0xffffffffu, blk_l == blk);
+      int n = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
       // a run belongs to the window that it starts in
       if (blk < 0 || blk == prev || blk >= a.num_blocks || (n == 1 && a.single_ctas > 0)) {
         if (blk >= a.num_blocks && threadIdx.x == 0) set_device_error(kDevBadIndex);
@@ -354,21 +354,22 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) rope_kv_append_fp
         t += blk < 0 ? 1 : n;
         continue;
       }
-      append_rows<D>(a, t, n, blk, slot, g0, g1, red);
+      int tr = lane < n ? t + lane : -1, at = slot;
+      if (n > kKvBlock) {  // more rows than slots: lane i takes the last row that names slot i
+        tr = -1;
+        at = blk * kKvBlock + lane;
+        n = 0;
+        for (int m = 32; m == 32; n += m) {
+          const int s2 = t + n + lane < T ? a.slots[t + n + lane] : -1;
+          const uint32_t in2 = __ballot_sync(0xffffffffu, s2 >= 0 && s2 / kKvBlock == blk);
+          m = in2 == 0xffffffffu ? 32 : __ffs(~in2) - 1;
+          for (int i = 0; i < m; ++i)
+            if (__shfl_sync(0xffffffffu, s2, i) == at) tr = t + n + i;
+        }
+      }
+      append_rows<D>(a, tr, at, blk, g0, g1, red);
       t += n;
       prev = blk;
-      // more than 16 neighbouring rows of one block name some slot twice: go on in
-      // order, as a later call would
-      while (n == kKvBlock && t < T) {
-        const int s2 = lane < kKvBlock && t + lane < T ? a.slots[t + lane] : -1;
-        const int b2 = s2 < 0 ? -1 : s2 / kKvBlock;
-        const uint32_t in2 = __ballot_sync(0xffffffffu, lane < kKvBlock && b2 == blk);
-        const int n2 = in2 == 0xffffu ? kKvBlock : __ffs(~in2) - 1;
-        if (n2 == 0) break;
-        append_rows<D>(a, t, n2, blk, s2, g0, g1, red);
-        t += n2;
-        if (n2 < kKvBlock) break;
-      }
     }
     return;
   }
