@@ -176,6 +176,17 @@ __device__ __forceinline__ float x_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+// Exponents x * kc + lv - mu of two raw scores.  The score is rounded before mu, a rounded
+// score itself, goes: with lv - mu formed first and one fma, scores from 2^28 on missed mu by
+// more than f16 weights bear.  Packed, the two steps issue as often as that one did.
+__device__ __forceinline__ void x_exponents(uint32_t x0, uint32_t x1, float kc, float lv, float mu,
+                                            float& y0, float& y1) {
+  asm("{\n.reg .b64 x, k, v, m;\n"
+      "mov.b64 x, {%2, %3};\nmov.b64 k, {%4, %4};\nmov.b64 v, {%5, %5};\nmov.b64 m, {%6, %6};\n"
+      "fma.rn.f32x2 x, x, k, v;\nadd.rn.f32x2 x, x, m;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(y0), "=f"(y1)
+      : "r"(x0), "r"(x1), "f"(kc), "f"(lv), "f"(-mu));
+}
 // Largest of 16 raw scores.
 __device__ __forceinline__ float x_max16(const uint32_t* x) {
   auto f = [&](int i) { return __uint_as_float(x[i]); };
@@ -604,12 +615,13 @@ __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const Pref
           float kc = k.x * c;
           kc = kc < FLT_MIN ? FLT_MIN : kc;
           kc = hidden ? 1.f : kc;
-          const float off = hidden ? 0.f : k.y - mu;
+          const float lv = hidden ? 0.f : k.y;
           float sa = 0.f, sb2 = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const float w0 = x_exp2(fmaf(__uint_as_float(x[i]), kc, off));
-            const float y1 = fmaf(__uint_as_float(x[i + 1]), kc, off);
+            float y0, y1;
+            x_exponents(x[i], x[i + 1], kc, lv, mu, y0, y1);
+            const float w0 = x_exp2(y0);
             const float w1 = (i & kXFmaMask) == kXFmaMask ? x_exp2_fma(y1) : x_exp2(y1);
             sa += w0;
             sb2 += w1;

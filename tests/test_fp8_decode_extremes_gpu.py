@@ -100,3 +100,27 @@ def test_values_of_both_ends_of_the_scale_range(cuda, hq, hkv, d, ctx):
     q = torch.randn(1, hq, d, device="cuda", generator=_gen(96)).bfloat16()
     q[:, :, 0] = 64.0
     _check(q, bt, [ctx], kf.to(FP8), ks, vc, vs, hq, hkv, d)
+
+
+@pytest.mark.parametrize("size", [4, 18, 24, 26, 30, 40, 60, 100])
+@pytest.mark.parametrize("ctx", [300, 9040])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_scores_of_any_size(cuda, hq, hkv, d, ctx, size):
+    """Scores of about 2^6 times 2^`size`: one key of each sequence stands above all others
+    and its value is the row."""
+    n = 3
+    bt, nb = _tables([ctx] * n, 6)
+    sign = torch.where(torch.rand(d, device="cuda", generator=_gen(97)) < 0.5, -1.0, 1.0)
+    vc, vs = _quantised(nb, hkv, d, 98, spread=2.0)
+    ks = torch.full((nb, hkv), 2.0 ** (size // 2), device="cuda")
+    for above, others in ((4.0, 0.5), (-0.5, -4.0)):
+        kf = others * torch.exp2(torch.randint(-1, 1, (nb, hkv, 16, d), device="cuda", generator=_gen(99)).float()) * sign
+        stars = [(4111 * b + 5) % ctx for b in range(n)]
+        for b, t in enumerate(stars):
+            kf[int(bt[b, t // 16]), :, t % 16] = above * sign
+        q = (2.0 ** (size - size // 2) * sign).expand(n, hq, d).bfloat16().contiguous()
+        out = _decode(q.flatten(1), bt, [ctx] * n, kf.to(FP8), ks, vc, vs, hq, hkv, d)
+        for b, t in enumerate(stars):
+            i = int(bt[b, t // 16])
+            want = (vc[i, :, t % 16].float() * vs[i][:, None]).repeat_interleave(hq // hkv, 0)
+            assert torch.equal(out[b].view(hq, d).float(), want), (above, b)

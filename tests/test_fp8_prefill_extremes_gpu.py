@@ -111,3 +111,27 @@ def test_values_of_both_ends_of_the_scale_range(cuda, hq, hkv, d, past, n):
     want, bound = _attend(q, kc, ks, vc, vs, bt[0], ctx, past + torch.arange(n, device="cuda"),
                           d ** -0.5, hkv)
     _near(out, want, bound, f"{past} + {n}")
+
+
+@pytest.mark.parametrize("size", [4, 18, 24, 26, 30, 40, 60, 100])
+@pytest.mark.parametrize("hq,hkv,d,ctx", [(4, 1, 128, 9040), (16, 8, 128, 300), (4, 2, 64, 300)])
+def test_scores_of_any_size(cuda, hq, hkv, d, ctx, size):
+    """Scores of about 2^6 times 2^`size`, positive and negative: one key of each sequence
+    stands above all others, and its value is the row (no sum, so nothing rounds: a code
+    times a power of two is a bf16 number)."""
+    n = 8 if ctx < 1000 else 2
+    bt, nb = _tables([ctx] * n, 6)
+    sign = torch.where(torch.rand(d, device="cuda", generator=_gen(97)) < 0.5, -1.0, 1.0)
+    vc, vs = _quantised(nb, hkv, d, 98, spread=2.0)
+    ks = torch.full((nb, hkv), 2.0 ** (size // 2), device="cuda")
+    for above, others in ((4.0, 0.5), (-0.5, -4.0)):
+        kf = others * torch.exp2(torch.randint(-1, 1, (nb, hkv, BS, d), device="cuda", generator=_gen(99)).float()) * sign
+        stars = [(37 * b + 5) % ctx if ctx < 1000 else 9000 - 4444 * b for b in range(n)]
+        for b, t in enumerate(stars):
+            kf[int(bt[b, t // BS]), :, t % BS] = above * sign
+        q = (2.0 ** (size - size // 2) * sign).expand(n, hq, d).bfloat16().contiguous()
+        out = _prefill(q.flatten(1), bt, [ctx] * n, [1] * n, kf.to(FP8), ks, vc, vs, hq, hkv, d)
+        for b, t in enumerate(stars):
+            i = int(bt[b, t // BS])
+            want = (vc[i, :, t % BS].float() * vs[i][:, None]).repeat_interleave(hq // hkv, 0)
+            assert torch.equal(out[b].view(hq, d).float(), want), (above, b)
