@@ -30,7 +30,8 @@
 // (4.9 TB/s; floor 68), 32 of up to 32k 202 us (5.6 TB/s; floor 171), also where the power
 // cap lowers the clock.  What bounds it now is the warps' chains of conversion, mma.sync and
 // exponentials, three warps per SM sub-partition: the same copies without them take 169 us as
-// 16 KB pieces.  Tried: such pieces by tensor copies from a loading warp 200 us (210 under
+// 16 KB pieces.  256 sequences of 1,000: groups of 4 heads 104 us (floor 80), groups of 16
+// 74 (40), head_dim 64 68 (40).  Tried: such pieces by tensor copies from a loading warp 200 us (210 under
 // the cap, 97 for the short sequences), 2 KB tensor copies per warp 221, 16 warps of fewer
 // registers 213.
 //
@@ -40,7 +41,10 @@
 //
 // Prefill (mma.sync, head_dim 64 and groups that the tensor-memory kernel does
 // not take): 64-key tiles staged as f16, rows masked causally at absolute
-// positions, the same weights w.  Three short prompts of a tiny model take 6.4 us.
+// positions, the same weights w.  Three short prompts of a tiny model take 6.4 us.  A tile is
+// staged, converted and multiplied by the same warps one after the other, which bounds it:
+// a fresh prompt of 4,000 takes 424 us with 32 heads of 64 on 8 (floor 40), 769 with 28 of
+// 128 on 4 (70).
 //
 // Semantics follow mu_inference/models/layers.py:700-723, as in attention.cu.
 #include <math.h>
@@ -66,7 +70,9 @@ struct DecodeFp8Shape {
   static constexpr int kStages = 2 + kAhead;  // cp.async ring per warp: two more in work
 };
 // Blocks of a run, at least: a shorter one costs more in its pair's join than it saves
-// (and a pair's partial results stay within kQdMaxParts).
+// (and a pair's partial results stay within kQdMaxParts: the bound of a launch lengthens its
+// runs from 24,000 tokens on, whatever the contexts are: 8 sequences of 4,000 take 27 us
+// under a bound of 4,368, 35 under 32,768 and 71 under 131,072).
 constexpr int kQdMinRun = 12;
 constexpr int kQdMaxParts = 127;   // partial results of a pair, at most
 constexpr int kQdFlatSeqs = 2048;  // sequences whose block counts a CTA adds up

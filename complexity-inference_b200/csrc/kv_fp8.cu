@@ -24,9 +24,11 @@
 // took 242 registers and left one CTA on an SM: 141 us for 8k rows.)  q rows are
 // rotated by further CTAs of the same launch.
 //
-// Bound: HBM by the bytes (q|k|v read, q and codes written), in fact latency: 8,000
-// rows of 32 + 16 heads of 128 take 52 us = 3.7 TB/s, the floor is 29; 256 decode
-// rows take 6.3 us, one 4.3 (an empty launch ~3).
+// Bound: HBM by the bytes (q|k|v read, q and codes written): the floor of 8,000 rows of
+// 32 + 16 heads of 128 is 29 us.  With QK-norm they take 52 us (3.7 TB/s), bound by
+// instructions: 36.7 M, issue slots 69 % busy, f64 sum of squares and products rounded one
+// by one; without it 46 us, 21.4 M and 50 %, waiting for loads.  256 decode rows take
+// 6.3 us, one 4.3 (an empty launch ~3): a dependent round of loads.
 //
 // The rotation is a*c - b*s with every product rounded (no fused multiply-add)
 // and the QK-norm factor is formed in f64: next to a rounding border of e4m3 the
@@ -485,9 +487,11 @@ extern "C" int muk_rope_kv_append_fp8(
   const int heads = kAppendThreads * 16 / (kKvBlock * head_dim);
   // Small steps are spread: a window's groups over as many CTAs, a q row a CTA, and rows
   // that are alone in their block get lanes of their own (a window would do 16 of them
-  // one after the other: 29 us for 256 decode rows).  In large steps, whose rows mostly
-  // have neighbours, a CTA keeps a window or 8 q rows and loads ahead: with a CTA for
-  // each group and q row, 8k rows took 61 us.
+  // one after the other: 29 us for 256 decode rows, and 6.3 so).  In large steps a CTA
+  // keeps a window or 8 q rows and loads ahead: with a CTA for each group and q row, 8k
+  // prompt rows took 61 us for 52.  Prompts change over evenly (1,024 rows 12.3 us, 1,025
+  // 10.3); decode rows pay for it in a large step, whose windows take their rows one after
+  // the other: 1,024 of them 12.4 us, 1,025 94, and 256 before 800 prompt rows 94.
   const bool large = num_tokens > 1024;
   a.groups = (2 * num_kv_heads + heads - 1) / heads;
   a.groups_per_cta = large ? a.groups : 1;

@@ -31,11 +31,12 @@
 // stay below 2^8 and O is rescaled in TMEM on those tiles alone (after P V of the
 // tile before has run); O and l use the same bound.
 //
-// Measured: a fresh prompt of 4,000 tokens (32 query heads on 8) 164 us = 800 TFLOP/s, floor
-// 80; four chunks of 300 to 700 rows behind 1,500 to 8,000 tokens (16 on 8) 139 us, floor 40:
+// Measured: a fresh prompt of 4,000 tokens (32 query heads on 8) 166 us = 790 TFLOP/s, floor
+// 80; four chunks of 300 to 700 rows behind 1,500 to 8,000 tokens (16 on 8) 142 us, floor 40:
 // there the CTA with the longest context sets the time, 1.1 us per 64 keys for the two query
-// tiles' chains softmax -> P V -> Q K^T, of which the multiplies are 0.76.  Bound: the
-// exponentials and the multiplies (N = 64) about equally.
+// tiles' chains softmax -> P V -> Q K^T, of which the multiplies are 0.76.  Bound: a row's
+// chain, one thread from load to maximum, exponentials, pack and store; no pipe is full
+// (tensor 39 % at N = 64, exponentials 30 %, issue slots 56 %).
 //
 // Few rows, long contexts (a short chunk behind a long past): where the query tiles would
 // fill less than half of the SMs, the CTAs of a cluster of 2, 4 or 8 share the keys of one,
@@ -254,7 +255,7 @@ __host__ __device__ constexpr uint32_t x_idesc(bool b_mn, int n) {
 }
 
 // Split: the CTAs of a cluster share a query tile's keys (otherwise one has all of them, in
-// code without the join: as one kernel for both, 4,000 tokens took 172 us for 164).
+// code without the join: as one kernel for both, 4,000 tokens took 5 % longer).
 template <bool Split>
 __global__ void __launch_bounds__(kXThreads, 1) prefill_fp8_tc_kernel(const PrefillFp8Args a) {
   // programmatic dependent launch: let the next kernel launch once every CTA

@@ -251,8 +251,8 @@ class PagedKVCache:
 
     # ---- forking and compacting ----------------------------------------------
     def _copy_blocks(self, src: List[int], dst: List[int]) -> None:
-        """Blocks ``src`` to ``dst`` in every layer, K and V, scales included: one
-        launch on the current stream (CPU pools: torch)."""
+        """Blocks ``src`` to ``dst`` in every layer, K and V, scales included: a launch
+        for every 256 of them on the current stream (CPU pools: torch)."""
         if not src:
             return
         if self.block_pool.is_cuda:
@@ -272,7 +272,7 @@ class PagedKVCache:
 
     def fork_many(self, pairs: Sequence[Tuple[str, str]]) -> bool:
         """Give each new request ``child`` the cached tokens of its ``parent``: full blocks
-        are shared, a partly filled last block is copied (all pairs' copies in one launch).
+        are shared, a partly filled last block is copied (all pairs' copies together).
         All-or-nothing: False, with nothing changed, when a parent is unknown, a child is
         known or named twice, or the pool has too few free blocks.  Call it between steps:
         the copy is ordered on the current stream."""
@@ -301,7 +301,7 @@ class PagedKVCache:
             return True
 
     def compact(self) -> int:
-        """Move the live blocks into the first ones of the pool (one launch on the current
+        """Move the live blocks into the first ones of the pool (copies on the current
         stream) and hand out the lowest free block first from then on; returns how many
         moved.  Call it between steps: slots reserved before it are no longer valid."""
         with self._lock:

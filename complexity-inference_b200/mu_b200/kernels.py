@@ -267,7 +267,8 @@ def rope_kv_append_fp8(qkv: torch.Tensor, positions: torch.Tensor, slot_mapping:
     """:func:`rope_kv_append` into the 8-bit cache: q rows (QK-norm, RoPE) go to
     ``q_out`` (None: in place), k and v rows are quantised into their blocks, whose
     scales grow as needed (a block starts anew with its row 0).  Rows of one block
-    must be neighbours in the batch; slots < 0 are skipped."""
+    must be neighbours in the batch with no skipped row between them; slots < 0 are
+    skipped.  A ``q_out`` that is not ``qkv`` does not overlap it."""
     name = "rope_kv_append_fp8"
     num_blocks, block_size = _check_cache_fp8(name, k_cache, v_cache, k_scale, v_scale,
                                               num_kv_heads, head_dim)

@@ -207,8 +207,11 @@ int muk_paged_prefill_attn(const void* q, int64_t q_stride, void* out, int64_t o
  * exponent), and where that grew its codes are rounded to the new scale.  The
  * codes are e4m3(x * 2^-e) and the scale 2^e.  A non-finite x makes the scale
  * NaN until the block starts anew.  Rows of one block must be neighbours in the
- * batch (a sequence's new tokens in order); of neighbouring rows naming one slot
- * the last counts.  qkv / q_out strides multiples of 8, buffers 16-byte aligned.
+ * batch, with no skipped row between them (a sequence's new tokens in order):
+ * otherwise two of them may rewrite the block at once, and its codes and scale
+ * are undefined.  Of neighbouring rows naming one slot the last counts.  q_out is
+ * qkv itself or does not overlap it.  qkv / q_out strides multiples of 8, buffers
+ * 16-byte aligned.
  * Bad positions and blocks latch device error 5 and are skipped. */
 int muk_rope_kv_append_fp8(const void* qkv, int64_t qkv_stride, void* q_out, int64_t q_out_stride,
                            const int32_t* positions, const int32_t* slot_mapping,
@@ -255,7 +258,8 @@ int muk_paged_prefill_attn_fp8(const void* q, int64_t q_stride, void* out, int64
  * a page, plane stride scale_plane_stride) in the same launch.  src and dst are
  * HOST arrays, read before the call returns (a captured graph keeps the pairs of
  * its capture).  No page may be a destination twice, nor a source and a
- * destination: MUK_ERR_INVALID_ARG, nothing copied.  Pools of any element type. */
+ * destination: MUK_ERR_INVALID_ARG, nothing copied.  Pools of any element type.
+ * One launch for every 256 pairs. */
 int muk_copy_pages(void* pool, int64_t plane_stride, int num_planes, int64_t page_bytes,
                    void* scales, int64_t scale_plane_stride, int scale_bytes, int num_blocks,
                    const int32_t* src, const int32_t* dst, int n, void* stream);
